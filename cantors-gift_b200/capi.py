@@ -80,6 +80,10 @@ class AttentionDesc(C.Structure):
                 ("reserved", C.c_int32)]
 
 
+class Grad(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("out_dtype", C.c_int32)]
+
+
 _vp, _vpp, _sz, _i, _i64 = C.c_void_p, C.POINTER(C.c_void_p), C.c_size_t, C.c_int, C.c_int64
 
 # name -> (restype, argtypes); exactly the declarations of include/cg_b200.h
@@ -112,6 +116,15 @@ SIGNATURES = {
     "cg_b200_layernorm": (_i, [_i, _vp, _vp, _vp, C.c_float, _vp, _i64, _i64, _vp]),
     "cg_b200_softmax_layernorm": (_i, [_i, _vp, _vp, _vp, C.c_float, _vp, _i64, _i64, _vp]),
     "cg_b200_reduce": (_i, [_i, _i, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "cg_b200_layernorm_forward": (_i, [_i, _i, _vp, _vp, _vp, C.c_float, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "cg_b200_layernorm_backward_workspace_bytes": (_i, [_i64, _i64, C.POINTER(_sz)]),
+    "cg_b200_layernorm_backward": (_i, [_i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "cg_b200_embedding": (_i, [_i, _i, _vp, _i64, _i64, _vp, _i, _i64, C.c_float, _vp, _vp]),
+    "cg_b200_embedding_backward_workspace_bytes": (_i, [_i64, _i64, _i64, C.POINTER(_sz)]),
+    "cg_b200_embedding_backward": (_i, [_i, _i, _vp, _vp, _i, _i64, C.c_float, _i64, _i, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "cg_b200_grad_norm_workspace_bytes": (_i, [_i64, C.POINTER(_sz)]),
+    "cg_b200_grad_norm": (_i, [C.POINTER(Grad), _i64, _vp, _vp, _sz, _vp]),
+    "cg_b200_clip_grad_norm": (_i, [C.POINTER(Grad), _i64, C.c_float, _vp, _vp, _sz, _vp]),
     "cg_b200_attention": (_i, [C.POINTER(AttentionDesc), _vp, _vp, _vp, _vp, _vp]),
     "cg_b200_gemm_workspace_bytes": (_i, [C.POINTER(GemmDesc), C.POINTER(_sz)]),
     "cg_b200_gemm": (_i, [C.POINTER(GemmDesc), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

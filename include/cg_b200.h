@@ -199,6 +199,46 @@ int cg_b200_softmax_layernorm(int dtype, const void* in, const void* gamma,
                               const void* beta, float eps, void* out, int64_t rows,
                               int64_t cols, void* stream);
 
+/* ---- layer norm for training ---------------------------------------------------------
+ * The reference describes layernorm's arithmetic (src/analysis/arithmetic_intensity.cpp:138-146) and has no gradient
+ * for it. With h = (x - mean) * rstd, g = dy * gamma and C = cols:
+ *   forward   y = h * gamma + beta, mean and rstd = 1 / sqrt(variance + eps) kept per row in fp32
+ *   backward  dx = rstd * (g - sum(g) / C - h * sum(g * h) / C), dgamma = sum over rows of dy * h, dbeta = sum over
+ *             rows of dy
+ * in, dout, out, din are [rows, cols] row-major contiguous of `dtype`; gamma, beta, dgamma, dbeta are [cols] of
+ * `param_dtype`, which is `dtype` or CG_B200_F32; mean, rstd are [rows] fp32. Any alignment down to the element size is
+ * taken; 16-byte packets are used when the [rows, cols] tensors start at the same offset from a 16-byte boundary. Math
+ * and sums are fp32, one rounding per result; the same inputs give the same bits on every call.
+ * Forward: gamma, beta, mean, rstd may be NULL; in == out is allowed. Backward: gamma may be NULL (taken as 1); din,
+ * dgamma, dbeta may each be NULL, not all three; din may be `dout` or `in` itself, not overlap them otherwise. rows == 0:
+ * dgamma and dbeta become zero. The workspace (256-byte aligned, contents undefined before and after) is used only
+ * when dgamma or dbeta is asked for; two calls that can run at the same time need one each. */
+int cg_b200_layernorm_forward(int dtype, int param_dtype, const void* in, const void* gamma, const void* beta, float eps,
+                              void* out, float* mean, float* rstd, int64_t rows, int64_t cols, void* stream);
+int cg_b200_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols, size_t* bytes);
+int cg_b200_layernorm_backward(int dtype, int param_dtype, const void* dout, const void* in, const void* gamma,
+                               const float* mean, const float* rstd, void* din, void* dgamma, void* dbeta, int64_t rows,
+                               int64_t cols, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- token embedding --------------------------------------------------------------------
+ * What makes the encoder block's [n, cols] input out of token ids, and the table's gradient (no counterpart in the
+ * reference). ids are `n` signed integers of id_bytes (4 or 8) bytes; an id outside [0, vocab) selects nothing.
+ *   forward   out[i] = scale * table[ids[i]], zero where the id selects nothing
+ *   backward  dtable[v] = scale * sum of dout[i] over the i with ids[i] == v; rows of `padding_id` (-1: none) and of ids
+ *             that do not occur are zero. With accumulate != 0 the sums are added to dtable instead, and rows without a
+ *             sum stay as they are.
+ * out / dout are `dtype`; table is `table_dtype`, dtable `grad_dtype`, each `dtype` or CG_B200_F32. All contiguous, any
+ * alignment down to the element size; 16-byte packets are used when cols and the bases allow them. The sums are fp32 in
+ * an order that the ids alone decide (the same inputs give the same bits on every call), rounded once.
+ * n, cols <= 2^31 - 1, vocab < 2^31 - 1. The workspace must be 256-byte aligned; its contents are undefined before and
+ * after, and two calls that can run at the same time need one each. */
+int cg_b200_embedding(int dtype, int table_dtype, const void* table, int64_t vocab, int64_t cols, const void* ids,
+                      int id_bytes, int64_t n, float scale, void* out, void* stream);
+int cg_b200_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t cols, size_t* bytes);
+int cg_b200_embedding_backward(int dtype, int grad_dtype, const void* dout, const void* ids, int id_bytes, int64_t n,
+                               float scale, int64_t padding_id, int accumulate, void* dtable, int64_t vocab, int64_t cols,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- reductions over a run of adjacent axes -----------------------------------------
  * Replaces the reduce lowering (VectorLoad, Reduce, VectorStore, src/lowering/tensor_to_codegen.cpp:332;
  * CGOpcode::Reduce is a comment in the PTX emitter, src/backend/ptx/ptx_emitter.cpp:136-142). Semantics
@@ -209,6 +249,28 @@ int cg_b200_softmax_layernorm(int dtype, const void* in, const void* gamma,
 enum cg_b200_reduce_op { CG_B200_REDUCE_SUM = 0, CG_B200_REDUCE_MAX = 1, CG_B200_REDUCE_MEAN = 2 };
 int cg_b200_reduce(int dtype, int op, const void* in, void* out, int64_t outer, int64_t reduce,
                    int64_t inner, void* stream);
+
+/* ---- gradient norm and clipping over a list of tensors ------------------------------------
+ * The reference's reductions take one tensor; these take a model's whole gradient list in a fixed number of launches.
+ *   norm = sqrt(sum over all tensors and elements of in^2)
+ *   clip: out = in * min(1, max_norm / (norm + 1e-6)), each rounded once to out_dtype
+ * `host_grads` is read before the call returns. A tensor is `n` contiguous elements of any alignment down to its element
+ * size; out_dtype is `dtype` or CG_B200_F32, out may be `in` itself when the types agree and otherwise must not overlap
+ * any input. No tensor may be written twice. *norm is fp32 on the device. Squares are summed in fp64 beyond 16-byte
+ * packets, in a fixed order; a list whose norm is infinite or not a number is scaled by the factor that the formula
+ * gives (0 or NaN). cg_b200_grad_norm ignores out, out_dtype. count <= 2^20; count == 0 gives norm 0. The workspace must
+ * be 16-byte aligned; two calls that can run at the same time need one each. */
+typedef struct cg_b200_grad {
+    const void* in;
+    void*       out;
+    int64_t     n;
+    int32_t     dtype, out_dtype;
+} cg_b200_grad;
+int cg_b200_grad_norm_workspace_bytes(int64_t count, size_t* bytes);
+int cg_b200_grad_norm(const cg_b200_grad* host_grads, int64_t count, float* norm, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int cg_b200_clip_grad_norm(const cg_b200_grad* host_grads, int64_t count, float max_norm, float* norm, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 /* ---- GEMM with fused epilogue -----------------------------------------------------
  * Replaces the matmul lowering (3 Const, 2 shared VectorLoad, K/k_tile FMA,
