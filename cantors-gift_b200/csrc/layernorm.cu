@@ -6,16 +6,19 @@
 //   backward  dx = rstd * (g - sum(g) / C - h * sum(g * h) / C)         (the two sums over the row)
 //             dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy
 //
-// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once. A row is read once into registers as 16-byte packets
-// (packet j of thread t is packet j * TPR + t), reduced by TPR threads - part of a warp, a warp or a whole CTA - and written; the next
-// row's packets are requested before the current row's reductions, so that loads are always in flight. In the backward pass each thread
-// adds its columns' share of dgamma and dbeta to fp32 registers over all rows that its CTA walks; the CTAs' sums go to the workspace and
-// a second kernel adds them up in a fixed order, so the result does not depend on timing.
+// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once. One CTA per SM walks the rows; its threads
+// form groups, a row (forward: two rows at once) to a group: eight threads, a warp, or up to 16 warps with a barrier of their own. A row is
+// 16-byte packets, packet j * TPR + t for thread t, copied asynchronously into shared memory up to three rows ahead: a thread copies and
+// reads its own packets only, so nothing but its own copies has to be waited for, and loads stay in flight while rows are reduced
+// without costing registers. In the backward pass each thread adds its columns' share of dgamma and dbeta to fp32 registers over all
+// rows of its group; the groups' sums are joined in shared memory, the CTAs' sums go to the workspace and a second kernel adds them up,
+// all in a fixed order, so the result does not depend on timing. Arithmetic is on fp32 pairs: with single instructions the backward
+// pass is bound by issue before it is bound by HBM.
 //
 // Rows whose width no packet divides start at a different offset from a 16-byte boundary each: `off` elements. The rows of one CTA are
-// gridDim.x apart, a multiple of the packet length, so they all share one offset: packets stay aligned, the first and the last of a row
-// are read and written element by element (never outside the row), and gamma / beta are kept in shared memory shifted by the same
-// offset. Tensors whose bases lie at different offsets, and rows too long for the registers, take the streaming kernels.
+// gridDim.x apart, a multiple of the packet length, so they all share one offset and a column stays with its thread. Packets stay aligned;
+// the first and the last of a row are read with what lies beside them in the tensor, which is dropped, and written element by element.
+// Tensors whose bases lie at different offsets, and rows too long for the registers, take the streaming kernels.
 #include <math.h>
 
 #include "common.cuh"
@@ -32,301 +35,523 @@ struct LnParams {
     float* rstd;
     float* part;         // backward: [gridDim.x][2][cols] fp32, or null when no weight gradient is asked for
     long long rows, cols;
+    long long edge_rows; // ragged rows at either end of the tensor whose outer packets may reach out of it
     int off0;            // elements from a 16-byte boundary to the first row, the same for every tensor
     float eps;
 };
 
-template <int TPR> constexpr int kLnThreads = TPR <= 32 ? 128 : TPR;   // threads of a CTA
+constexpr int kLnThreads = 512;   // of a CTA at most: 128 registers each
+constexpr int kLnWarps = kLnThreads / 32;
 
-// Sum of two values over the TPR threads that share a row; every thread gets it. Two scratch halves take turns, so one barrier per call
-// is enough.
-template <int TPR>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2* scratch, int& phase) {
-    constexpr int W = TPR < 32 ? TPR : 32;
-    const unsigned mask = W == 32 ? 0xffffffffu : ((1u << W) - 1u) << (threadIdx.x & 31 & ~(W - 1));
+// Sums of N values over the threads that share a row (8 lanes of a warp when SUB, else `warps` warps); every thread gets them. The warps
+// of a group meet at barrier `bar`; two scratch halves take turns, so one barrier per call is enough.
+template <int N> struct alignas(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) LnSums {
+    float v[N];
+};
+template <int N>
+__device__ __forceinline__ void ln_add_across(LnSums<N>& s, unsigned mask, int o) {
+    LnSums<N> t;
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-        v.x += __shfl_xor_sync(mask, v.x, o);
-        v.y += __shfl_xor_sync(mask, v.y, o);
-    }
-    if constexpr (TPR > 32) {
-        constexpr int N = TPR / 32;
-        float2* s = scratch + (phase & 1) * N;
-        phase ^= 1;
-        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = s[threadIdx.x & (N - 1)];
+    for (int i = 0; i < N; ++i) t.v[i] = __shfl_xor_sync(mask, s.v[i], o);
 #pragma unroll
-        for (int o = N / 2; o > 0; o >>= 1) {
-            v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-            v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    for (int i = 0; i < N; ++i) s.v[i] += t.v[i];
+}
+template <bool SUB, int N>
+__device__ __forceinline__ void row_sum(LnSums<N>& s, LnSums<N>* scratch, int& phase, int bar, int warps) {
+    const unsigned mask = SUB ? 0xffu << (threadIdx.x & 24) : 0xffffffffu;
+#pragma unroll
+    for (int o = SUB ? 4 : 16; o > 0; o >>= 1) ln_add_across(s, mask, o);
+    if (!SUB && warps > 1) {
+        const int lane = threadIdx.x & 31;
+        LnSums<N>* at = scratch + phase;
+        phase ^= 16;
+        if (lane == 0) at[(threadIdx.x >> 5) % warps] = s;
+        asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
+        if (warps <= 4) {
+            s = at[0];
+            for (int w = 1; w < warps; ++w)
+#pragma unroll
+                for (int i = 0; i < N; ++i) s.v[i] += at[w].v[i];
+            return;
         }
-    }
-    return v;
-}
-
-// Packet k of a row whose columns start `off` elements behind the packet boundary `row0`; elements outside the row read as zero.
-template <typename T, bool RAGGED>
-__device__ __forceinline__ Vec16<T> ln_load(const T* row0, int k, int off, int cols) {
-    constexpr int L = Vec16<T>::N;
-    if constexpr (!RAGGED) {
-        return ld_stream(row0 + k * L);
-    } else {
-        const int c0 = k * L - off;
-        if (c0 >= 0 && c0 + L <= cols) return ld_stream(row0 + k * L);
-        Vec16<T> v;
+        s = at[lane < warps ? lane : 0];
 #pragma unroll
-        for (int l = 0; l < L; ++l) v.v[l] = c0 + l >= 0 && c0 + l < cols ? row0[k * L + l] : Elem<T>::from_f32(0.0f);
-        return v;
+        for (int i = 0; i < N; ++i) s.v[i] = lane < warps ? s.v[i] : 0.0f;
+        if (warps > 8) ln_add_across(s, 0xffffffffu, 8);
+        ln_add_across(s, 0xffffffffu, 4);
+        ln_add_across(s, 0xffffffffu, 2);
+        ln_add_across(s, 0xffffffffu, 1);
+        // lanes 0 .. 7 (0 .. 15) hold the sums, the others added zeros
+#pragma unroll
+        for (int i = 0; i < N; ++i) s.v[i] = __shfl_sync(0xffffffffu, s.v[i], 0);
     }
 }
 
-template <typename T, bool RAGGED>
-__device__ __forceinline__ void ln_store(T* row0, int k, int off, int cols, const Vec16<T>& v) {
+__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most `stages` - 1 of this thread's groups are under way
+__device__ __forceinline__ void copy_wait(int stages) {
+    if (stages >= 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Where a ragged row's ends lie: `head` columns of packet 0 and all from `tail` on in packet `last` belong to its neighbours. A CTA's rows
+// all share this, and a thread with neither packet has nothing to do about it.
+struct LnEnds {
+    bool first, last;   // this thread has packet 0, the last packet
+    int last_j;         // as its packet last_j
+    int head, tail;
+};
+template <int L>
+__device__ __forceinline__ LnEnds ln_ends(int off, int cols, int n_pkt, int tpr, int lane) {
+    LnEnds e;
+    e.head = off;
+    e.tail = off + cols - (n_pkt - 1) * L;
+    e.last_j = (n_pkt - 1) / tpr;
+    e.first = lane == 0 && e.head > 0;
+    e.last = lane == n_pkt - 1 - e.last_j * tpr && e.tail < L;
+    return e;
+}
+// Clears what belongs to the neighbours: `keep` has all bits set for each of this thread's columns that is in the row. Only the threads with
+// a row's ends come here, but their group waits for them: a read and an AND per value, nothing that depends on anything.
+template <int L, int CH>
+__device__ __forceinline__ void ln_clear_ends(const uint4* keep, float2 (&x)[CH][L / 2]) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+        for (int l = 0; l < L / 2; l += 2) {
+            const uint4 m = keep[(j * L + 2 * l) / 4];
+            x[j][l].x = __uint_as_float(__float_as_uint(x[j][l].x) & m.x);
+            x[j][l].y = __uint_as_float(__float_as_uint(x[j][l].y) & m.y);
+            x[j][l + 1].x = __uint_as_float(__float_as_uint(x[j][l + 1].x) & m.z);
+            x[j][l + 1].y = __uint_as_float(__float_as_uint(x[j][l + 1].y) & m.w);
+        }
+}
+// Before the first use: the masks of a thread with an end (its own only)
+template <int L, int CH>
+__device__ __forceinline__ void ln_write_keep(uint32_t* keep, int c_lane, int c_step, int cols) {
+    for (int i = 0; i < CH * L; ++i) {
+        const int c = c_lane + i / L * c_step + i % L;
+        keep[i] = c >= 0 && c < cols ? 0xffffffffu : 0u;
+    }
+}
+// Packet j of a row, by a thread that has an end of it
+template <typename T>
+__device__ __forceinline__ void ln_store_end(T* to, const LnEnds& e, int j, const Vec16<T>& v) {
     constexpr int L = Vec16<T>::N;
-    const int c0 = k * L - off;
-    if (!RAGGED || (c0 >= 0 && c0 + L <= cols)) {
-        st_stream(row0 + k * L, v);
+    const int head = j == 0 && e.first ? e.head : 0, tail = j == e.last_j && e.last ? e.tail : L;
+    if (head == 0 && tail == L) {
+        st_stream(to, v);
     } else {
 #pragma unroll
         for (int l = 0; l < L; ++l)
-            if (c0 + l >= 0 && c0 + l < cols) row0[k * L + l] = v.v[l];
+            if (l >= head && l < tail) to[l] = v.v[l];
+    }
+}
+// A packet into shared memory. The ends of a ragged row come with what lies beside them in the tensor; where that would reach out of the
+// tensor (`careful`: the rows at its ends) only what is inside is read.
+template <typename T>
+__device__ __forceinline__ void ln_copy(Vec16<T>* to, const T* from, bool careful, const void* tensor, long long size) {
+    constexpr int L = Vec16<T>::N;
+    const T* base = static_cast<const T*>(tensor);
+    if (!careful || (from >= base && from + L <= base + size)) {
+        copy16_async(to, from);
+    } else {
+        Vec16<T> v;
+#pragma unroll
+        for (int l = 0; l < L; ++l) v.v[l] = from + l >= base && from + l < base + size ? from[l] : Elem<T>::from_f32(0.0f);
+        *to = v;
     }
 }
 
-// L parameters of packet k: from global memory (L1 keeps them) where packets and columns coincide, from the shifted copy otherwise.
-template <typename TP, int L, bool RAGGED>
-__device__ __forceinline__ void ln_param(const TP* p, const float* shifted, int k, float (&f)[L]) {
-    if constexpr (RAGGED) {
+// L values as fp32 pairs
+template <typename T>
+__device__ __forceinline__ void ln_pairs(const Vec16<T>& v, float2* f) {
+    float t[Vec16<T>::N];
+    unpack16<T>(v, t);
 #pragma unroll
-        for (int l = 0; l < L; l += 4) {
-            const float4 t = *reinterpret_cast<const float4*>(shifted + k * L + l);
-            f[l] = t.x; f[l + 1] = t.y; f[l + 2] = t.z; f[l + 3] = t.w;
+    for (int i = 0; i < Vec16<T>::N / 2; ++i) f[i] = make_float2(t[2 * i], t[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ Vec16<T> ln_packet(const float2* f) {
+    float t[Vec16<T>::N];
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::N / 2; ++i) {
+        t[2 * i] = f[i].x;
+        t[2 * i + 1] = f[i].y;
+    }
+    return pack16<T>(t);
+}
+
+// The L parameters of the packet with the columns c0 ..; `none` without parameters and outside the row.
+template <typename TP, int L, bool RAGGED>
+__device__ __forceinline__ void ln_param(const TP* p, int c0, int cols, float none, float2 (&f)[L / 2]) {
+    if (!p) {
+#pragma unroll
+        for (int l = 0; l < L / 2; ++l) f[l] = make_float2(none, none);
+    } else if constexpr (RAGGED) {
+#pragma unroll
+        for (int l = 0; l < L / 2; ++l) {
+            f[l].x = c0 + 2 * l >= 0 && c0 + 2 * l < cols ? Elem<TP>::to_f32(p[c0 + 2 * l]) : none;
+            f[l].y = c0 + 2 * l + 1 >= 0 && c0 + 2 * l + 1 < cols ? Elem<TP>::to_f32(p[c0 + 2 * l + 1]) : none;
         }
     } else {
         constexpr int M = Vec16<TP>::N;   // M <= L: the parameters have the rows' type or fp32
 #pragma unroll
-        for (int l = 0; l < L; l += M) {
-            float t[M];
-            unpack16<TP>(ld_keep(p + k * L + l), t);
-#pragma unroll
-            for (int i = 0; i < M; ++i) f[l + i] = t[i];
-        }
+        for (int l = 0; l < L; l += M) ln_pairs<TP>(ld_keep(p + c0 + l), f + l / 2);
     }
 }
 
-template <typename TP>
-__device__ __forceinline__ void ln_stage(float* shifted, const TP* p, int off, int cols, int padded) {
-    for (int i = threadIdx.x; i < padded; i += blockDim.x) {
-        const int c = i - off;
-        shifted[i] = c >= 0 && c < cols ? Elem<TP>::to_f32(p[c]) : 0.0f;
-    }
-}
+// How a CTA's threads share its rows (the launch's choice, see ln_launch)
+struct LnShape {
+    int tpr;        // threads per row: 8 when SUB, else a multiple of 32
+    int groups;     // rows at a time
+    int stages;     // rows ahead
+};
 
-template <typename T, typename TP, int TPR, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kLnThreads<TPR>) ln_fwd_kernel(const __grid_constant__ LnParams p) {
-    constexpr int L = Vec16<T>::N, THREADS = kLnThreads<TPR>, G = THREADS / TPR;
+// CH packets per thread; the parameters stay in registers. A group takes R rows at a time: the dependent reductions of a row are latency,
+// which the rows share.
+template <typename T, typename TP, int CH, int R, bool SUB, bool RAGGED>
+__global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_constant__ LnParams p, const LnShape sh) {
+    constexpr int L = Vec16<T>::N;
     extern __shared__ float4 ln_smem4[];
-    __shared__ float2 scratch[TPR > 32 ? TPR / 16 : 1];
-    float* sg = reinterpret_cast<float*>(ln_smem4);
+    __shared__ LnSums<R> scratch_all[SUB ? 1 : kLnWarps * 32];
+    __shared__ uint4 keep_all[RAGGED ? kLnThreads / (SUB ? 8 : 32) * 2 : 1][RAGGED ? CH * L / 4 : 1];
+    const int tpr = SUB ? 8 : sh.tpr, group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr, warps = tpr >> 5;
+    LnSums<R>* scratch = scratch_all + (SUB ? 0 : group * 32);
     int phase = 0;
-    const int cols = (int)p.cols, lane = threadIdx.x % TPR;
+    const int cols = (int)p.cols;
     // all rows of this CTA share the offset of row blockIdx.x: gridDim.x is a multiple of L when rows are ragged
     const int off = RAGGED ? (int)((p.off0 + (long long)blockIdx.x * cols) % L) : 0;
-    const int n_pkt = (off + cols + L - 1) / L, padded = n_pkt * L;
-    float* sb = sg + padded;
-    const TP* gamma = static_cast<const TP*>(p.gamma);
-    const TP* beta = static_cast<const TP*>(p.beta);
-    if constexpr (RAGGED) {
-        if (gamma) ln_stage(sg, gamma, off, cols, padded);
-        if (beta) ln_stage(sb, beta, off, cols, padded);
-        __syncthreads();
+    const int n_pkt = (off + cols + L - 1) / L;
+    Vec16<T>* ring = reinterpret_cast<Vec16<T>*>(ln_smem4) + threadIdx.x;   // this thread's slots: [stages][R][CH], kLnThreads apart
+    const long long step = (long long)gridDim.x * sh.groups, first = (long long)group * gridDim.x + blockIdx.x;
+    const int left = first < p.rows ? (int)((p.rows - 1 - first) / step) + 1 : 0;   // rows of this group
+    const int c_lane = lane * L - off, c_step = tpr * L;
+    auto live = [&](int j) { return j * tpr + lane < n_pkt; };
+    const T* src = static_cast<const T*>(p.in) + first * p.cols + c_lane;   // of the next row to fetch
+    int to_fetch = left;
+    long long at = first;
+    auto fetch = [&](Vec16<T>* slot) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (to_fetch-- > 0) {
+                const bool careful = RAGGED && (at < p.edge_rows || at >= p.rows - p.edge_rows);
+#pragma unroll
+                for (int j = 0; j < CH; ++j)
+                    if (live(j)) ln_copy<T>(slot + (r * CH + j) * kLnThreads, src + j * c_step, careful, p.in, p.rows * p.cols);
+                src += step * p.cols;
+                at += step;
+            } else if (r > 0) {
+#pragma unroll
+                for (int j = 0; j < CH; ++j) slot[(r * CH + j) * kLnThreads] = Vec16<T>{};
+            }
+        copy_commit();
+    };
+    // what a thread does not fetch it reads as zero: the arithmetic below asks nothing about packets and rows that are not there
+    for (int i = 0; i < sh.stages * R; ++i)
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+            if (!live(j)) ring[(i * CH + j) * kLnThreads] = Vec16<T>{};
+    for (int i = 0; i < sh.stages; ++i) fetch(ring + i * R * CH * kLnThreads);
+    const LnEnds ends = ln_ends<L>(off, cols, n_pkt, tpr, lane);
+    const bool has_end = RAGGED && (ends.first || ends.last);
+    uint4* keep = keep_all[RAGGED ? group * 2 + (ends.first ? 0 : 1) : 0];
+    if (has_end) ln_write_keep<L, CH>(reinterpret_cast<uint32_t*>(keep), c_lane, c_step, cols);
+    float2 g[CH][L / 2], b[CH][L / 2];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+        ln_param<TP, L, RAGGED>(live(j) ? static_cast<const TP*>(p.gamma) : nullptr, c_lane + j * c_step, cols, 1.0f, g[j]);
+        ln_param<TP, L, RAGGED>(live(j) ? static_cast<const TP*>(p.beta) : nullptr, c_lane + j * c_step, cols, 0.0f, b[j]);
     }
     const float inv_cols = 1.0f / (float)cols;
-    const long long step = (long long)gridDim.x * G;
-    long long row = (long long)(threadIdx.x / TPR) * gridDim.x + blockIdx.x;
-    Vec16<T> raw[CH], nxt[CH];
-    auto fetch = [&](Vec16<T> (&v)[CH], long long r) {
-        const T* row0 = static_cast<const T*>(p.in) + r * p.cols - off;
+    T* dst = static_cast<T*>(p.out) + first * p.cols + c_lane;
+    long long row = first;
+    int stage = 0;
+    for (int i = 0; i < left; i += R) {
+        Vec16<T>* slot = ring + stage * R * CH * kLnThreads;
+        stage = stage + 1 == sh.stages ? 0 : stage + 1;
+        copy_wait(sh.stages);
+        float2 x[R][CH][L / 2];
+        LnSums<R> s;
 #pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (j * TPR + lane < n_pkt) v[j] = ln_load<T, RAGGED>(row0, j * TPR + lane, off, cols);
-    };
-    if (row < p.rows) fetch(raw, row);
-    for (; row < p.rows; row += step) {
-        if (row + step < p.rows) fetch(nxt, row + step);
-        float x[CH][L];
-        float2 s = make_float2(0.0f, 0.0f);
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (j * TPR + lane < n_pkt) {
-                unpack16<T>(raw[j], x[j]);
+            for (int j = 0; j < CH; ++j) ln_pairs<T>(slot[(r * CH + j) * kLnThreads], x[r][j]);
+        fetch(slot);
+        if (has_end) {
 #pragma unroll
-                for (int l = 0; l < L; ++l) s.x += x[j][l];
-            }
-        const float mean = row_sum2<TPR>(s, scratch, phase).x * inv_cols;
-        s.x = 0.0f;
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (j * TPR + lane < n_pkt) {
-                const int c0 = (j * TPR + lane) * L - off;
-#pragma unroll
-                for (int l = 0; l < L; ++l) {
-                    x[j][l] -= mean;
-                    if (RAGGED && (c0 + l < 0 || c0 + l >= cols)) x[j][l] = 0.0f;
-                    s.x = fmaf(x[j][l], x[j][l], s.x);
-                }
-            }
-        const float rstd = 1.0f / sqrtf(row_sum2<TPR>(s, scratch, phase).x * inv_cols + p.eps);
-        if (lane == 0) {
-            if (p.mean) p.mean[row] = mean;
-            if (p.rstd) p.rstd[row] = rstd;
+            for (int r = 0; r < R; ++r) ln_clear_ends<L, CH>(keep, x[r]);
         }
-        T* out0 = static_cast<T*>(p.out) + row * p.cols - off;
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            const int k = j * TPR + lane;
-            if (k < n_pkt) {
-                float f[L];
-#pragma unroll
-                for (int l = 0; l < L; ++l) x[j][l] *= rstd;
-                if (gamma) {
-                    ln_param<TP, L, RAGGED>(gamma, sg, k, f);
-#pragma unroll
-                    for (int l = 0; l < L; ++l) x[j][l] *= f[l];
-                }
-                if (beta) {
-                    ln_param<TP, L, RAGGED>(beta, sb, k, f);
-#pragma unroll
-                    for (int l = 0; l < L; ++l) x[j][l] += f[l];
-                }
-                ln_store<T, RAGGED>(out0, k, off, cols, pack16<T>(x[j]));
-            }
-            raw[j] = nxt[j];
-        }
-    }
-}
-
-template <typename T, typename TP, int TPR, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kLnThreads<TPR>) ln_bwd_kernel(const __grid_constant__ LnParams p) {
-    constexpr int L = Vec16<T>::N, THREADS = kLnThreads<TPR>, G = THREADS / TPR;
-    extern __shared__ float4 ln_smem4[];
-    __shared__ float2 scratch[TPR > 32 ? TPR / 16 : 1];
-    float* sg = reinterpret_cast<float*>(ln_smem4);
-    int phase = 0;
-    const int cols = (int)p.cols, lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    const int off = RAGGED ? (int)((p.off0 + (long long)blockIdx.x * cols) % L) : 0;
-    const int n_pkt = (off + cols + L - 1) / L, padded = n_pkt * L;
-    const TP* gamma = static_cast<const TP*>(p.gamma);
-    if constexpr (RAGGED) {
-        if (gamma) ln_stage(sg, gamma, off, cols, padded);
-        __syncthreads();
-    }
-    const float inv_cols = 1.0f / (float)cols;
-    const long long step = (long long)gridDim.x * G;
-    long long row = (long long)group * gridDim.x + blockIdx.x;
-    float dg[CH][L], db[CH][L];
-#pragma unroll
-    for (int j = 0; j < CH; ++j)
-#pragma unroll
-        for (int l = 0; l < L; ++l) dg[j][l] = db[j][l] = 0.0f;
-    Vec16<T> xr[CH], yr[CH], xn[CH], yn[CH];
-    float mean, rstd, mean_n = 0.0f, rstd_n = 0.0f;
-    auto fetch = [&](Vec16<T> (&xv)[CH], Vec16<T> (&yv)[CH], float& m, float& r, long long at) {
-        const T* x0 = static_cast<const T*>(p.in) + at * p.cols - off;
-        const T* y0 = static_cast<const T*>(p.dout) + at * p.cols - off;
-        m = p.mean[at];
-        r = p.rstd[at];
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (j * TPR + lane < n_pkt) {
-                xv[j] = ln_load<T, RAGGED>(x0, j * TPR + lane, off, cols);
-                yv[j] = ln_load<T, RAGGED>(y0, j * TPR + lane, off, cols);
-            }
-    };
-    if (row < p.rows) fetch(xr, yr, mean, rstd, row);
-    for (; row < p.rows; row += step) {
-        if (row + step < p.rows) fetch(xn, yn, mean_n, rstd_n, row + step);
-        float2 s = make_float2(0.0f, 0.0f);   // sum(g), sum(g h)
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            const int k = j * TPR + lane;
-            if (k < n_pkt) {
-                float x[L], y[L], g[L];
-                unpack16<T>(xr[j], x);
-                unpack16<T>(yr[j], y);
-                if (gamma) ln_param<TP, L, RAGGED>(gamma, sg, k, g);
-#pragma unroll
-                for (int l = 0; l < L; ++l) {
-                    const float h = (x[l] - mean) * rstd;
-                    dg[j][l] = fmaf(y[l], h, dg[j][l]);
-                    db[j][l] += y[l];
-                    const float t = gamma ? y[l] * g[l] : y[l];
-                    s.x += t;
-                    s.y = fmaf(t, h, s.y);
-                }
-            }
-        }
-        s = row_sum2<TPR>(s, scratch, phase);
-        const float a = s.x * inv_cols, b = s.y * inv_cols;
-        T* out0 = static_cast<T*>(p.out) + row * p.cols - off;
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            const int k = j * TPR + lane;
-            if (k < n_pkt && p.out) {
-                float x[L], y[L], g[L];
-                unpack16<T>(xr[j], x);
-                unpack16<T>(yr[j], y);
-                if (gamma) ln_param<TP, L, RAGGED>(gamma, sg, k, g);
-#pragma unroll
-                for (int l = 0; l < L; ++l) {
-                    const float h = (x[l] - mean) * rstd;
-                    const float t = gamma ? y[l] * g[l] : y[l];
-                    x[l] = rstd * (t - a - h * b);
-                }
-                ln_store<T, RAGGED>(out0, k, off, cols, pack16<T>(x));
-            }
-            xr[j] = xn[j];
-            yr[j] = yn[j];
-        }
-        mean = mean_n;
-        rstd = rstd_n;
-    }
-    if (!p.part) return;
-    // this CTA's sums: the row groups' registers are added in the order of the groups
-    float* part = p.part + (long long)blockIdx.x * 2 * p.cols;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        if constexpr (G == 1) {
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const int k = j * TPR + lane;
-                if (k < n_pkt) {
-#pragma unroll
-                    for (int l = 0; l < L; ++l) {
-                        const int c = k * L + l - off;
-                        if (!RAGGED || (c >= 0 && c < cols)) part[(long long)w * cols + c] = w ? db[j][l] : dg[j][l];
-                    }
-                }
-            }
-        } else {
-            constexpr int SPAN = TPR * CH * L;   // the columns a group covers
-            float* sum = sg;                      // G * SPAN floats; gamma's copy is not needed any more
-            __syncthreads();
+        for (int r = 0; r < R; ++r) {
+            float2 t = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int j = 0; j < CH; ++j)
 #pragma unroll
-                for (int l = 0; l < L; l += 4) {
-                    const float* f = w ? &db[j][l] : &dg[j][l];
-                    *reinterpret_cast<float4*>(sum + group * SPAN + (j * TPR + lane) * L + l) = make_float4(f[0], f[1], f[2], f[3]);
-                }
-            __syncthreads();
-            for (int c = threadIdx.x; c < cols; c += THREADS) {
-                float t = 0.0f;
+                for (int l = 0; l < L / 2; ++l) t = __fadd2_rn(t, x[r][j][l]);
+            s.v[r] = t.x + t.y;
+        }
+        row_sum<SUB>(s, scratch, phase, group + 1, warps);
+        float mean[R];
 #pragma unroll
-                for (int g = 0; g < G; ++g) t += sum[g * SPAN + c + off];
-                part[(long long)w * cols + c] = t;
+        for (int r = 0; r < R; ++r) {
+            mean[r] = s.v[r] * inv_cols;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const float neg = live(j) ? -mean[r] : 0.0f;   // what is not there stays zero
+#pragma unroll
+                for (int l = 0; l < L / 2; ++l) x[r][j][l] = __fadd2_rn(x[r][j][l], make_float2(neg, neg));
             }
+        }
+        if (has_end) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) ln_clear_ends<L, CH>(keep, x[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float2 t = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+#pragma unroll
+                for (int l = 0; l < L / 2; ++l) t = __ffma2_rn(x[r][j][l], x[r][j][l], t);
+            s.v[r] = t.x + t.y;
+        }
+        row_sum<SUB>(s, scratch, phase, group + 1, warps);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r == 0 || i + r < left) {
+                const float rstd = rsqrtf(s.v[r] * inv_cols + p.eps);
+                if (lane == 0) {
+                    if (p.mean) p.mean[row] = mean[r];
+                    if (p.rstd) p.rstd[row] = rstd;
+                }
+                const float2 rstd2 = make_float2(rstd, rstd);
+                Vec16<T> y[CH];
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+#pragma unroll
+                    for (int l = 0; l < L / 2; ++l) x[r][j][l] = __ffma2_rn(__fmul2_rn(x[r][j][l], rstd2), g[j][l], b[j][l]);
+                    y[j] = ln_packet<T>(x[r][j]);
+                }
+                if (!has_end) {
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (live(j)) st_stream(dst + j * c_step, y[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (live(j)) ln_store_end(dst + j * c_step, ends, j, y[j]);
+                }
+                row += step;
+                dst += step * p.cols;
+            }
+    }
+}
+
+// KEEP: the parameters and, from the first to the second pass over a row, its g and h stay in registers (up to 16 columns per thread);
+// otherwise both passes read the row from shared memory and the parameters anew (32 columns, one row at a time).
+template <typename T, typename TP, int CH, int R, bool SUB, bool RAGGED>
+__global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_constant__ LnParams p, const LnShape sh) {
+    constexpr int L = Vec16<T>::N;
+    constexpr bool KEEP = CH * L <= 16;
+    static_assert(KEEP || R == 1, "rows at a time are kept in registers");
+    extern __shared__ float4 ln_smem4[];
+    __shared__ LnSums<2 * R> scratch_all[SUB ? 1 : kLnWarps * 32];
+    __shared__ uint4 keep_all[RAGGED ? kLnThreads / (SUB ? 8 : 32) * 2 : 1][RAGGED ? CH * L / 4 : 1];
+    const int tpr = SUB ? 8 : sh.tpr, group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr, warps = tpr >> 5;
+    LnSums<2 * R>* scratch = scratch_all + (SUB ? 0 : group * 32);
+    int phase = 0;
+    const int cols = (int)p.cols;
+    const int off = RAGGED ? (int)((p.off0 + (long long)blockIdx.x * cols) % L) : 0;
+    const int n_pkt = (off + cols + L - 1) / L;
+    Vec16<T>* ring = reinterpret_cast<Vec16<T>*>(ln_smem4) + threadIdx.x;   // this thread's slots: [stages][R][x, dy][CH], kLnThreads apart
+    const TP* gamma = static_cast<const TP*>(p.gamma);
+    const long long step = (long long)gridDim.x * sh.groups, first = (long long)group * gridDim.x + blockIdx.x;
+    const int left = first < p.rows ? (int)((p.rows - 1 - first) / step) + 1 : 0;
+    const int c_lane = lane * L - off, c_step = tpr * L;
+    auto live = [&](int j) { return j * tpr + lane < n_pkt; };
+    const T* x_src = static_cast<const T*>(p.in) + first * p.cols + c_lane;
+    const T* y_src = static_cast<const T*>(p.dout) + first * p.cols + c_lane;
+    int to_fetch = left;
+    long long at = first;
+    auto fetch = [&](Vec16<T>* slot) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (to_fetch-- > 0) {
+                const bool careful = RAGGED && (at < p.edge_rows || at >= p.rows - p.edge_rows);
+#pragma unroll
+                for (int j = 0; j < CH; ++j)
+                    if (live(j)) {
+                        ln_copy<T>(slot + (r * 2 * CH + j) * kLnThreads, x_src + j * c_step, careful, p.in, p.rows * p.cols);
+                        ln_copy<T>(slot + (r * 2 * CH + CH + j) * kLnThreads, y_src + j * c_step, careful, p.dout, p.rows * p.cols);
+                    }
+                x_src += step * p.cols;
+                y_src += step * p.cols;
+                at += step;
+            } else if (r > 0) {
+#pragma unroll
+                for (int j = 0; j < 2 * CH; ++j) slot[(r * 2 * CH + j) * kLnThreads] = Vec16<T>{};
+            }
+        copy_commit();
+    };
+    for (int i = 0; i < sh.stages * R * 2; ++i)
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+            if (!live(j)) ring[(i * CH + j) * kLnThreads] = Vec16<T>{};
+    for (int i = 0; i < sh.stages; ++i) fetch(ring + i * R * 2 * CH * kLnThreads);
+    float mean_n[R], rstd_n[R];   // of the next rows, read in time; zero for rows that are not there
+    auto statistics = [&](int i) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            mean_n[r] = rstd_n[r] = 0.0f;
+            if (i + r < left) {
+                mean_n[r] = p.mean[first + (i + r) * step];
+                rstd_n[r] = p.rstd[first + (i + r) * step];
+            }
+        }
+    };
+    statistics(0);
+    const LnEnds ends = ln_ends<L>(off, cols, n_pkt, tpr, lane);
+    const bool has_end = RAGGED && (ends.first || ends.last);
+    uint4* keep = keep_all[RAGGED ? group * 2 + (ends.first ? 0 : 1) : 0];
+    if (has_end) ln_write_keep<L, CH>(reinterpret_cast<uint32_t*>(keep), c_lane, c_step, cols);
+    const float inv_cols = 1.0f / (float)cols;
+    float2 dg[CH][L / 2], db[CH][L / 2], g[KEEP ? CH : 1][L / 2];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+#pragma unroll
+        for (int l = 0; l < L / 2; ++l) dg[j][l] = db[j][l] = make_float2(0.0f, 0.0f);
+        if (KEEP) ln_param<TP, L, RAGGED>(live(j) ? gamma : nullptr, c_lane + j * c_step, cols, 1.0f, g[KEEP ? j : 0]);
+    }
+    T* dst = static_cast<T*>(p.out) + first * p.cols + c_lane;
+    int stage = 0;
+    for (int i = 0; i < left; i += R) {
+        Vec16<T>* slot = ring + stage * R * 2 * CH * kLnThreads;
+        stage = stage + 1 == sh.stages ? 0 : stage + 1;
+        float mean[R], rstd[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            mean[r] = mean_n[r];
+            rstd[r] = rstd_n[r];
+        }
+        statistics(i + R);
+        copy_wait(sh.stages);
+        constexpr int K = KEEP ? CH : 1;   // packets held at a time
+        float2 h[R][K][L / 2], t[R][K][L / 2];
+        // x and dy of packets j0 .. j0 + K - 1 of row r, into h and t
+        auto read = [&](int r, int j0) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                ln_pairs<T>(slot[(r * 2 * CH + j0 + j) * kLnThreads], h[r][j]);
+                ln_pairs<T>(slot[(r * 2 * CH + CH + j0 + j) * kLnThreads], t[r][j]);
+            }
+        };
+        auto clear = [&](int r, int j0) {
+            ln_clear_ends<L, K>(keep + j0 * L / 4, h[r]);
+            ln_clear_ends<L, K>(keep + j0 * L / 4, t[r]);
+        };
+        // What is not there has x = dy = 0 and so adds nothing: to the sums over rows as dy, to the sums over columns as g.
+        LnSums<2 * R> s;   // sum(g), sum(g h) of each row
+        if (KEEP) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) read(r, 0);
+            fetch(slot);
+            if (has_end) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) clear(r, 0);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float2 neg_mean = make_float2(-mean[r], -mean[r]), rstd2 = make_float2(rstd[r], rstd[r]);
+            float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                constexpr int Z = KEEP ? 1 : 0;
+                if (!KEEP) {
+                    read(r, j);
+                    if (has_end) clear(r, j);
+                    ln_param<TP, L, RAGGED>(live(j) ? gamma : nullptr, c_lane + j * c_step, cols, 1.0f, g[0]);
+                }
+#pragma unroll
+                for (int l = 0; l < L / 2; ++l) {
+                    float2 &hl = h[r][j * Z][l], &tl = t[r][j * Z][l];
+                    hl = __fmul2_rn(__fadd2_rn(hl, neg_mean), rstd2);
+                    dg[j][l] = __ffma2_rn(tl, hl, dg[j][l]);
+                    db[j][l] = __fadd2_rn(db[j][l], tl);
+                    tl = __fmul2_rn(tl, g[j * Z][l]);
+                    s1 = __fadd2_rn(s1, tl);
+                    s2 = __ffma2_rn(tl, hl, s2);
+                }
+            }
+            s.v[2 * r] = s1.x + s1.y;
+            s.v[2 * r + 1] = s2.x + s2.y;
+        }
+        row_sum<SUB>(s, scratch, phase, group + 1, warps);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r == 0 || i + r < left) {
+                const float a = -rstd[r] * (s.v[2 * r] * inv_cols), b = -rstd[r] * (s.v[2 * r + 1] * inv_cols);
+                const float2 a2 = make_float2(a, a), b2 = make_float2(b, b), neg_mean = make_float2(-mean[r], -mean[r]),
+                             rstd2 = make_float2(rstd[r], rstd[r]);
+                if (p.out) {
+                    Vec16<T> o[CH];
+#pragma unroll
+                    for (int j = 0; j < CH; ++j) {
+                        constexpr int Z = KEEP ? 1 : 0;
+                        if constexpr (!KEEP) {
+                            read(r, j);
+                            ln_param<TP, L, RAGGED>(live(j) ? gamma : nullptr, c_lane + j * c_step, cols, 1.0f, g[0]);
+#pragma unroll
+                            for (int l = 0; l < L / 2; ++l) {
+                                h[0][0][l] = __fmul2_rn(__fadd2_rn(h[0][0][l], neg_mean), rstd2);
+                                t[0][0][l] = __fmul2_rn(t[0][0][l], g[0][l]);
+                            }
+                        }
+                        float2 f[L / 2];
+#pragma unroll
+                        for (int l = 0; l < L / 2; ++l) f[l] = __ffma2_rn(t[r][j * Z][l], rstd2, __ffma2_rn(h[r][j * Z][l], b2, a2));
+                        o[j] = ln_packet<T>(f);
+                    }
+                    if (!has_end) {
+#pragma unroll
+                        for (int j = 0; j < CH; ++j)
+                            if (live(j)) st_stream(dst + j * c_step, o[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < CH; ++j)
+                            if (live(j)) ln_store_end(dst + j * c_step, ends, j, o[j]);
+                    }
+                }
+                dst += step * p.cols;
+            }
+        if (!KEEP) fetch(slot);
+    }
+    if (!p.part) return;
+    // this CTA's sums: the groups' registers are added in the order of the groups
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    float* sum = reinterpret_cast<float*>(ln_smem4);
+    float* part = p.part + (long long)blockIdx.x * 2 * p.cols;
+    const int span = tpr * CH * L;   // the columns a group covers
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+#pragma unroll
+            for (int l = 0; l < L / 2; l += 2) {
+                const float2 u = w ? db[j][l] : dg[j][l], v = w ? db[j][l + 1] : dg[j][l + 1];
+                *reinterpret_cast<float4*>(sum + group * span + (j * tpr + lane) * L + 2 * l) = make_float4(u.x, u.y, v.x, v.y);
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+            float t = 0.0f;
+            for (int q = 0; q < sh.groups; ++q) t += sum[q * span + c + off];
+            part[(long long)w * cols + c] = t;
         }
     }
 }
@@ -334,22 +559,24 @@ __global__ void __launch_bounds__(kLnThreads<TPR>) ln_bwd_kernel(const __grid_co
 // ---- rows of any length and alignment --------------------------------------------------------------
 template <typename T, typename TP>
 __global__ void __launch_bounds__(256) ln_fwd_stream_kernel(const __grid_constant__ LnParams p) {
-    __shared__ float2 scratch[16];
+    __shared__ LnSums<1> scratch[32];
     int phase = 0;
     const TP* gamma = static_cast<const TP*>(p.gamma);
     const TP* beta = static_cast<const TP*>(p.beta);
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T* in = static_cast<const T*>(p.in) + row * p.cols;
         T* out = static_cast<T*>(p.out) + row * p.cols;
-        float2 s = make_float2(0.0f, 0.0f);
-        for (long long c = threadIdx.x; c < p.cols; c += 256) s.x += Elem<T>::to_f32(in[c]);
-        const float mean = row_sum2<256>(s, scratch, phase).x / (float)p.cols;
-        s.x = 0.0f;
+        LnSums<1> s{0.0f};
+        for (long long c = threadIdx.x; c < p.cols; c += 256) s.v[0] += Elem<T>::to_f32(in[c]);
+        row_sum<false>(s, scratch, phase, 1, 8);
+        const float mean = s.v[0] / (float)p.cols;
+        s.v[0] = 0.0f;
         for (long long c = threadIdx.x; c < p.cols; c += 256) {
             const float d = Elem<T>::to_f32(in[c]) - mean;
-            s.x = fmaf(d, d, s.x);
+            s.v[0] = fmaf(d, d, s.v[0]);
         }
-        const float rstd = 1.0f / sqrtf(row_sum2<256>(s, scratch, phase).x / (float)p.cols + p.eps);
+        row_sum<false>(s, scratch, phase, 1, 8);
+        const float rstd = rsqrtf(s.v[0] / (float)p.cols + p.eps);
         if (threadIdx.x == 0) {
             if (p.mean) p.mean[row] = mean;
             if (p.rstd) p.rstd[row] = rstd;
@@ -366,7 +593,7 @@ __global__ void __launch_bounds__(256) ln_fwd_stream_kernel(const __grid_constan
 
 template <typename T, typename TP>
 __global__ void __launch_bounds__(256) ln_bwd_stream_kernel(const __grid_constant__ LnParams p) {
-    __shared__ float2 scratch[16];
+    __shared__ LnSums<2> scratch[32];
     int phase = 0;
     const TP* gamma = static_cast<const TP*>(p.gamma);
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -374,15 +601,15 @@ __global__ void __launch_bounds__(256) ln_bwd_stream_kernel(const __grid_constan
         const T* y = static_cast<const T*>(p.dout) + row * p.cols;
         T* out = static_cast<T*>(p.out) + row * p.cols;
         const float mean = p.mean[row], rstd = p.rstd[row];
-        float2 s = make_float2(0.0f, 0.0f);
+        LnSums<2> s{0.0f, 0.0f};
         for (long long c = threadIdx.x; c < p.cols; c += 256) {
             const float h = (Elem<T>::to_f32(x[c]) - mean) * rstd;
             const float t = Elem<T>::to_f32(y[c]) * (gamma ? Elem<TP>::to_f32(gamma[c]) : 1.0f);
-            s.x += t;
-            s.y = fmaf(t, h, s.y);
+            s.v[0] += t;
+            s.v[1] = fmaf(t, h, s.v[1]);
         }
-        s = row_sum2<256>(s, scratch, phase);
-        const float a = s.x / (float)p.cols, b = s.y / (float)p.cols;
+        row_sum<false>(s, scratch, phase, 1, 8);
+        const float a = s.v[0] / (float)p.cols, b = s.v[1] / (float)p.cols;
         for (long long c = threadIdx.x; c < p.cols; c += 256) {
             const float h = (Elem<T>::to_f32(x[c]) - mean) * rstd;
             const float t = Elem<T>::to_f32(y[c]) * (gamma ? Elem<TP>::to_f32(gamma[c]) : 1.0f);
@@ -420,48 +647,60 @@ __global__ void __launch_bounds__(256) ln_bwd_columns_kernel(const __grid_consta
 
 // dgamma (blockIdx.y == 0) and dbeta (1): the sums of `parts` rows of the workspace, in a fixed order
 template <typename TP>
-__global__ void __launch_bounds__(256) ln_weight_grad_kernel(const float* part, long long parts, long long cols, TP* dgamma, TP* dbeta) {
-    __shared__ float sum[8][32];
+__global__ void __launch_bounds__(512) ln_weight_grad_kernel(const float* part, long long parts, long long cols, TP* dgamma, TP* dbeta) {
+    __shared__ float sum[16][32];
     TP* out = blockIdx.y ? dbeta : dgamma;
     const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
     float s = 0.0f;
     if (out && c < cols) {
         const float* q = part + blockIdx.y * cols + c;
-#pragma unroll 4
-        for (long long i = threadIdx.y; i < parts; i += 8) s += q[i * 2 * cols];
+#pragma unroll 8
+        for (long long i = threadIdx.y; i < parts; i += 16) s += q[i * 2 * cols];
     }
     sum[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && out && c < cols) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += sum[i][threadIdx.x];
+        for (int i = 1; i < 16; ++i) s += sum[i][threadIdx.x];
         out[c] = Elem<TP>::from_f32(s);
     }
 }
 
 // CTAs that the backward pass starts at most: their sums are the workspace
 static long long ln_max_parts(long long rows) {
-    const long long cap = (long long)sm_count() * 3;
+    const long long cap = sm_count();
     return ((rows < cap ? rows : cap) + 7) / 8 * 8;
 }
 
-template <typename T, typename TP, int TPR, int CH, bool BWD>
+template <typename T, typename TP, int CH, int R, bool SUB, bool BWD>
 static int ln_launch(const LnParams& p, bool ragged, int* parts, cudaStream_t s) {
-    constexpr int L = Vec16<T>::N, THREADS = kLnThreads<TPR>, G = THREADS / TPR;
-    // Backward CTAs are resident all at once (three of 128 threads per SM, or 384 threads' worth); the forward pass keeps more in flight.
-    const long long cap = BWD ? (long long)sm_count() * (THREADS >= 512 ? 1 : THREADS == 256 ? 2 : 3) : (long long)sm_count() * (2048 / THREADS);
-    long long grid = (p.rows + G - 1) / G;
-    if (grid > cap) grid = cap;
-    if (ragged) grid = (grid + L - 1) / L * L;
-    const int padded = (int)((p.cols + 2 * L - 2) / L) * L;   // of the largest offset
-    size_t smem = ragged ? (size_t)padded * 4 * (BWD ? 1 : 2) : 0;
-    if (BWD && G > 1 && smem < (size_t)G * TPR * CH * L * 4) smem = (size_t)G * TPR * CH * L * 4;
+    constexpr int L = Vec16<T>::N;
+    const int padded = (int)((p.cols + (ragged ? 2 * L - 2 : 0)) / L) * L;   // columns with the largest offset, in whole packets
+    LnShape sh;
+    sh.tpr = SUB ? 8 : ((padded + CH * L - 1) / (CH * L) + 31) / 32 * 32;
+    // few rows: fewer groups per CTA, so that every SM has some
+    const long long sms = sm_count(), want = (p.rows + sms - 1) / sms;
+    const int most = kLnThreads / sh.tpr;
+    sh.groups = (int)(want < most ? want : most);
+    if (SUB) sh.groups = (sh.groups + 3) / 4 * 4;   // whole warps
+    const int threads = sh.groups * sh.tpr;
+    const size_t row = (size_t)R * CH * kLnThreads * 16 * (BWD ? 2 : 1);
+    sh.stages = 3;
+    while (row * sh.stages > 208 * 1024) --sh.stages;   // of 227 KB, with the static scratch and what the system keeps per CTA
+    size_t smem = row * sh.stages;
+    const size_t join = (size_t)threads * CH * L * 4;
+    if (BWD && smem < join) smem = join;
+    long long grid = (p.rows + sh.groups - 1) / sh.groups;
+    if (grid > sms) grid = sms;
+    if (ragged) grid = grid >= L ? grid / L * L : L;   // down: a CTA more than fits would be a wave of its own
     if (parts) *parts = (int)grid;
-#define CGB_LN_GO(R)                                                                                                        \
+#define CGB_LN_GO(M)                                                                                                        \
     {                                                                                                                       \
-        auto k = BWD ? ln_bwd_kernel<T, TP, TPR, CH, R> : ln_fwd_kernel<T, TP, TPR, CH, R>;                                 \
-        if (smem > 48 * 1024) CGB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));    \
-        k<<<(unsigned)grid, THREADS, smem, s>>>(p);                                                                         \
+        void (*k)(const LnParams, const LnShape);                                                                           \
+        if constexpr (BWD) k = ln_bwd_kernel<T, TP, CH, R, SUB, M>;                                                         \
+        else k = ln_fwd_kernel<T, TP, CH, R, SUB, M>;                                                                       \
+        if (smem > 32 * 1024) CGB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));    \
+        k<<<(unsigned)grid, threads, smem, s>>>(p, sh);                                                                     \
     }
     if (ragged) CGB_LN_GO(true) else CGB_LN_GO(false)
 #undef CGB_LN_GO
@@ -472,22 +711,19 @@ static int ln_launch(const LnParams& p, bool ragged, int* parts, cudaStream_t s)
 // Whether all tensors start the same number of elements behind a 16-byte boundary
 static bool ln_congruent(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
 
-// The register kernels' variants: threads per row and packets per thread by the packets of a row. -1: none, the streaming kernels take it.
+// The register kernels' variants: packets per thread by the length of a row. -1: none, the streaming kernels take it.
 template <typename T, typename TP, bool BWD>
 static int ln_registers(LnParams p, bool params_aligned, int* parts, cudaStream_t s) {
     constexpr int L = Vec16<T>::N;
     if (!ln_congruent(p.in, p.out ? p.out : p.in) || (BWD && !ln_congruent(p.in, p.dout))) return -1;
     p.off0 = (int)((reinterpret_cast<uintptr_t>(p.in) & 15) / sizeof(T));
+    p.edge_rows = (L + p.cols - 1) / p.cols;
     const bool ragged = p.off0 != 0 || p.cols % L != 0 || !params_aligned;
-    const long long n = ragged ? (p.cols + 2 * L - 2) / L : p.cols / L;
-    if (n <= 8) return ln_launch<T, TP, 8, 1, BWD>(p, ragged, parts, s);
-    if (n <= 32) return ln_launch<T, TP, 32, 1, BWD>(p, ragged, parts, s);
-    if (n <= 64) return ln_launch<T, TP, 32, 2, BWD>(p, ragged, parts, s);
-    if (n <= 128) return ln_launch<T, TP, 32, 4, BWD>(p, ragged, parts, s);
-    if (n <= 256) return ln_launch<T, TP, 128, 2, BWD>(p, ragged, parts, s);
-    if (n <= 512) return ln_launch<T, TP, 128, 4, BWD>(p, ragged, parts, s);
-    if (n <= 1024) return ln_launch<T, TP, 256, 4, BWD>(p, ragged, parts, s);
-    if (n <= 2048) return ln_launch<T, TP, 512, 4, BWD>(p, ragged, parts, s);
+    const long long n = p.cols + (ragged ? 2 * L - 2 : 0);   // elements that the packets of a row cover at most
+    if (n <= 64) return ln_launch<T, TP, 8 / L, BWD ? 1 : 2, true, BWD>(p, ragged, parts, s);
+    if (n <= 256) return ln_launch<T, TP, 8 / L, BWD ? 1 : 2, false, BWD>(p, ragged, parts, s);
+    if (n <= 16 * kLnThreads) return ln_launch<T, TP, 16 / L, BWD ? 1 : 2, false, BWD>(p, ragged, parts, s);
+    if (n <= 32 * kLnThreads) return ln_launch<T, TP, 32 / L, 1, false, BWD>(p, ragged, parts, s);
     return -1;
 }
 
@@ -526,7 +762,7 @@ static int ln_backward(const LnParams& p, void* dgamma, void* dbeta, cudaStream_
         }
     }
     if (dgamma || dbeta) {
-        ln_weight_grad_kernel<TP><<<dim3((unsigned)((p.cols + 31) / 32), 2), dim3(32, 8), 0, s>>>(p.part, parts, p.cols, static_cast<TP*>(dgamma),
+        ln_weight_grad_kernel<TP><<<dim3((unsigned)((p.cols + 31) / 32), 2), dim3(32, 16), 0, s>>>(p.part, parts, p.cols, static_cast<TP*>(dgamma),
                                                                                                   static_cast<TP*>(dbeta));
         CGB_CUDA(cudaGetLastError());
     }

@@ -103,9 +103,9 @@ def reduce(x, op, axes, keep_dims=False, out=None, stream=None):
 # These run on the device their tensors lie on (which need not be the current one) and on `stream` if one is given; what
 # they allocate - results and workspaces, new ones for every call - then belongs to that stream. Inputs made on another
 # stream are the caller's to order, as with every torch call.
-def _call_context(stream, x):
+def _elsewhere(x, stream):
     """None when the call can go ahead as it is, else the context that makes x's device (and `stream`) current."""
-    index = x.device.index
+    index = x.get_device()
     if stream is not None:
         if stream.device != x.device:
             raise ValueError(f"stream is on {stream.device}, tensors are on {x.device}")
@@ -115,10 +115,21 @@ def _call_context(stream, x):
 
 
 def _require_one_device(x, *tensors):
-    _require_cuda(x, *tensors)
+    if not x.is_cuda or not x.is_contiguous():
+        raise ValueError("cg_b200 ops take contiguous CUDA tensors")
+    index = x.get_device()
     for t in tensors:
-        if t is not None and t.device != x.device:
-            raise ValueError(f"tensors are on {x.device} and {t.device}")
+        if t is not None and (t.get_device() != index or not t.is_contiguous()):
+            raise ValueError(f"cg_b200 ops take contiguous CUDA tensors on one device ({x.device})")
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(index):
+    """The current stream's handle: torch.cuda.current_stream(index).cuda_stream without building a Stream object (3.5 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _dtype_code(dtype):
@@ -129,11 +140,17 @@ def _dtype_code(dtype):
 
 
 def _param_code(x, *params):
-    """The type that gamma, beta and their gradients share: x's own or fp32."""
-    kinds = {t.dtype for t in params if t is not None} or {x.dtype}
-    if len(kinds) != 1 or not kinds <= {x.dtype, torch.float32}:
-        raise ValueError(f"parameters must all have dtype {x.dtype} or float32")
-    return DTYPE_OF_TORCH[kinds.pop()]
+    """The type that gamma, beta and their gradients share: x's own or fp32. Their shape: [cols]."""
+    kind, shape = None, x.shape[-1:]
+    for t in params:
+        if t is None:
+            continue
+        kind = t.dtype if kind is None else kind
+        if t.dtype != kind or (kind != x.dtype and kind != torch.float32):
+            raise ValueError(f"parameters must all have dtype {x.dtype} or all float32")
+        if t.shape != shape:
+            raise ValueError(f"parameters must be {tuple(shape)}, got {tuple(t.shape)}")
+    return _dtype_code(x.dtype if kind is None else kind)
 
 
 def _rows_cols(x):
@@ -144,7 +161,7 @@ def _rows_cols(x):
 
 
 def _check_like(t, shape, dtype, what):
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{what} must be {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
 
 
@@ -152,23 +169,27 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, r
     """layernorm over the last axis that keeps its statistics: (y, mean, rstd), mean and rstd fp32 of shape x.shape[:-1].
     gamma, beta: [cols] of x's dtype or fp32, each may be None. `out` may be x."""
     _require_one_device(x, gamma, beta, out, mean, rstd)
-    ctx = _call_context(stream, x)
+    ctx = _elsewhere(x, stream)
     if ctx is not None:
         with ctx:
             return layernorm_forward(x, gamma, beta, eps, out, mean, rstd)
     dt, pt = _dtype_code(x.dtype), _param_code(x, gamma, beta)
     rows, cols = _rows_cols(x)
-    for t, what in ((gamma, "gamma"), (beta, "beta")):
-        if t is not None:
-            _check_like(t, (cols,), t.dtype, what)
-    _check_like(out, x.shape, x.dtype, "out")
-    _check_like(mean, x.shape[:-1], torch.float32, "mean")
-    _check_like(rstd, x.shape[:-1], torch.float32, "rstd")
-    out = torch.empty_like(x) if out is None else out
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if mean is None else mean
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if rstd is None else rstd
-    check(lib().cg_b200_layernorm_forward(dt, pt, _ptr(x), _ptr(gamma), _ptr(beta), eps, _ptr(out), _ptr(mean), _ptr(rstd),
-                                          rows, cols, _stream()), "layernorm_forward")
+    shape, lead = x.shape, x.shape[:-1]
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _check_like(out, shape, x.dtype, "out")
+    if mean is None:
+        mean = torch.empty(lead, dtype=torch.float32, device=x.device)
+    else:
+        _check_like(mean, lead, torch.float32, "mean")
+    if rstd is None:
+        rstd = torch.empty_like(mean)
+    else:
+        _check_like(rstd, lead, torch.float32, "rstd")
+    check(lib().cg_b200_layernorm_forward(dt, pt, x.data_ptr(), _addr(gamma), _addr(beta), eps, out.data_ptr(), mean.data_ptr(),
+                                          rstd.data_ptr(), rows, cols, _raw_stream(x.get_device())), "layernorm_forward")
     return out, mean, rstd
 
 
@@ -176,20 +197,19 @@ def layernorm_backward(dy, x, mean, rstd, gamma=None, bias=True, dx=None, dgamma
     """Gradients of layernorm_forward: (dx, dgamma, dbeta). dgamma and dbeta are made when gamma is given (dbeta unless
     bias=False) and have gamma's dtype; buffers passed as dgamma / dbeta are filled in any case. `dx` may be dy or x."""
     _require_one_device(x, dy, mean, rstd, gamma, dx, dgamma, dbeta)
-    ctx = _call_context(stream, x)
+    ctx = _elsewhere(x, stream)
     if ctx is not None:
         with ctx:
             return layernorm_backward(dy, x, mean, rstd, gamma, bias, dx, dgamma, dbeta)
     dt, pt = _dtype_code(x.dtype), _param_code(x, gamma, dgamma, dbeta)
     rows, cols = _rows_cols(x)
     _check_like(dy, x.shape, x.dtype, "dy")
-    _check_like(dx, x.shape, x.dtype, "dx")
     _check_like(mean, x.shape[:-1], torch.float32, "mean")
     _check_like(rstd, x.shape[:-1], torch.float32, "rstd")
-    for t, what in ((gamma, "gamma"), (dgamma, "dgamma"), (dbeta, "dbeta")):
-        if t is not None:
-            _check_like(t, (cols,), t.dtype, what)
-    dx = torch.empty_like(x) if dx is None else dx
+    if dx is None:
+        dx = torch.empty_like(x)
+    else:
+        _check_like(dx, x.shape, x.dtype, "dx")
     if gamma is not None:
         dgamma = torch.empty_like(gamma) if dgamma is None else dgamma
         dbeta = torch.empty_like(gamma) if dbeta is None and bias else dbeta
@@ -199,8 +219,9 @@ def layernorm_backward(dy, x, mean, rstd, gamma=None, bias=True, dx=None, dgamma
         check(lib().cg_b200_layernorm_backward_workspace_bytes(rows, cols, C.byref(need)), "layernorm_backward_workspace_bytes")
         ws_bytes = need.value
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-    check(lib().cg_b200_layernorm_backward(dt, pt, _ptr(dy), _ptr(x), _ptr(gamma), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dgamma),
-                                           _ptr(dbeta), rows, cols, _ptr(ws), ws_bytes, _stream()), "layernorm_backward")
+    check(lib().cg_b200_layernorm_backward(dt, pt, dy.data_ptr(), x.data_ptr(), _addr(gamma), mean.data_ptr(), rstd.data_ptr(),
+                                           dx.data_ptr(), _addr(dgamma), _addr(dbeta), rows, cols, _addr(ws), ws_bytes,
+                                           _raw_stream(x.get_device())), "layernorm_backward")
     return dx, dgamma, dbeta
 
 
@@ -208,29 +229,33 @@ _ID_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
 def _id_bytes(ids):
-    if ids.dtype not in _ID_BYTES:
+    width = _ID_BYTES.get(ids.dtype)
+    if width is None:
         raise ValueError(f"ids must be int32 or int64, got {ids.dtype}")
-    return _ID_BYTES[ids.dtype]
+    return width
 
 
 def embedding(table, ids, scale=1.0, dtype=None, out=None, stream=None):
     """scale * table[ids] of shape ids.shape + (cols,): the activations that a token sequence starts from. `dtype` (default:
     the table's) may be bf16 or f16 with an fp32 table. An id outside the table gives a row of zeros."""
     _require_one_device(table, ids, out)
-    ctx = _call_context(stream, table)
+    ctx = _elsewhere(table, stream)
     if ctx is not None:
         with ctx:
             return embedding(table, ids, scale, dtype, out)
     if table.dim() != 2:
         raise ValueError("table must be [vocab, cols]")
-    dtype = (table.dtype if out is None else out.dtype) if dtype is None else dtype
+    if dtype is None:
+        dtype = table.dtype if out is None else out.dtype
     dt, tt, idb = _dtype_code(dtype), _dtype_code(table.dtype), _id_bytes(ids)
     vocab, cols = table.shape
     shape = (*ids.shape, cols)
-    _check_like(out, shape, dtype, "out")
-    out = torch.empty(shape, dtype=dtype, device=table.device) if out is None else out
-    check(lib().cg_b200_embedding(dt, tt, _ptr(table), vocab, cols, _ptr(ids), idb, ids.numel(), scale, _ptr(out), _stream()),
-          "embedding")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=table.device)
+    else:
+        _check_like(out, shape, dtype, "out")
+    check(lib().cg_b200_embedding(dt, tt, table.data_ptr(), vocab, cols, ids.data_ptr(), idb, ids.numel(), scale, out.data_ptr(),
+                                  _raw_stream(table.get_device())), "embedding")
     return out
 
 
@@ -239,7 +264,7 @@ def embedding_backward(dy, ids, vocab, scale=1.0, padding_id=None, dtype=None, o
     sum of dy over the places of ids that hold v, zero for ids that do not occur and for `padding_id`. accumulate=True adds
     to `out` instead. The same inputs give the same bits on every call."""
     _require_one_device(dy, ids, out)
-    ctx = _call_context(stream, dy)
+    ctx = _elsewhere(dy, stream)
     if ctx is not None:
         with ctx:
             return embedding_backward(dy, ids, vocab, scale, padding_id, dtype, out, accumulate)
@@ -247,94 +272,83 @@ def embedding_backward(dy, ids, vocab, scale=1.0, padding_id=None, dtype=None, o
         raise ValueError(f"dy must be ids.shape + (cols,): got {tuple(dy.shape)} for ids {tuple(ids.shape)}")
     if accumulate and out is None:
         raise ValueError("accumulate=True needs the buffer to add to as `out`")
-    dtype = (dy.dtype if out is None else out.dtype) if dtype is None else dtype
+    if dtype is None:
+        dtype = dy.dtype if out is None else out.dtype
     dt, gt, idb = _dtype_code(dy.dtype), _dtype_code(dtype), _id_bytes(ids)
     n, cols = ids.numel(), dy.shape[-1]
-    _check_like(out, (vocab, cols), dtype, "out")
-    out = torch.empty((vocab, cols), dtype=dtype, device=dy.device) if out is None else out
+    if out is None:
+        out = torch.empty((vocab, cols), dtype=dtype, device=dy.device)
+    else:
+        _check_like(out, (vocab, cols), dtype, "out")
     need = C.c_size_t(0)
     check(lib().cg_b200_embedding_backward_workspace_bytes(n, vocab, cols, C.byref(need)), "embedding_backward_workspace_bytes")
     ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
-    check(lib().cg_b200_embedding_backward(dt, gt, _ptr(dy), _ptr(ids), idb, n, scale, -1 if padding_id is None else padding_id,
-                                           int(accumulate), _ptr(out), vocab, cols, _ptr(ws), need.value, _stream()),
-          "embedding_backward")
+    check(lib().cg_b200_embedding_backward(dt, gt, dy.data_ptr(), ids.data_ptr(), idb, n, scale,
+                                           -1 if padding_id is None else padding_id, int(accumulate), out.data_ptr(), vocab, cols,
+                                           ws.data_ptr(), need.value, _raw_stream(dy.get_device())), "embedding_backward")
     return out
 
 
-def _grad_list(grads, outs):
-    """The C ABI's table of a list of tensors. Empty tensors may be among them; no tensor may be written twice."""
-    if len(outs) != len(grads):
-        raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
-    table = (capi.Grad * max(1, len(grads)))()
-    device, written = None, set()
-    for e, g, o in zip(table, grads, outs):
-        if not g.is_cuda or not g.is_contiguous() or (o is not g and not (o.is_cuda and o.is_contiguous())):
-            raise ValueError("cg_b200 ops take contiguous CUDA tensors")
-        device = g.device if device is None else device
-        if g.device != device or o.device != device:
-            raise ValueError("the tensors of a list must be on one device")
-        if o is not g and o.shape != g.shape:
-            raise ValueError(f"output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
-        e.in_, e.out, e.n = g.data_ptr(), o.data_ptr(), g.numel()
-        e.dtype, e.out_dtype = _dtype_code(g.dtype), _dtype_code(o.dtype)
-        if e.n:
-            if e.out in written:
-                raise ValueError("a tensor is in the list twice")
-            written.add(e.out)
-    for e in table:
-        if e.n and e.in_ != e.out and e.in_ in written:
-            raise ValueError("an output is another gradient of the list")
-    return table, device
+def _grad_table(grads, outs):
+    """The C ABI's table of a list of tensors, four 64-bit words each (cg_b200_grad). Empty tensors may be among them."""
+    index, words = grads[0].get_device(), []
+    for g, o in zip(grads, outs):
+        if index < 0 or g.get_device() != index or not g.is_contiguous():
+            raise ValueError("cg_b200 ops take contiguous CUDA tensors on one device")
+        if o is not g:
+            if o.get_device() != index or not o.is_contiguous():
+                raise ValueError("cg_b200 ops take contiguous CUDA tensors on one device")
+            if o.shape != g.shape:
+                raise ValueError(f"output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
+        words += (g.data_ptr(), o.data_ptr(), g.numel(), _dtype_code(g.dtype) | _dtype_code(o.dtype) << 32)
+    return (C.c_int64 * len(words))(*words), words
 
 
 def grad_norm(grads, norm=None, stream=None):
     """sqrt of the sum of squares over all tensors of `grads`: a 0-dim fp32 tensor on their device."""
-    return _norm_of(list(grads), None, None, norm, stream)
+    return _norm_call(list(grads), None, None, norm, stream)
 
 
 def clip_grad_norm(grads, max_norm, out=None, norm=None, stream=None):
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)) and returns their norm before it (0-dim fp32, on the device;
     nothing waits for the GPU). In place, or into `out`: tensors of the same shapes, each of its gradient's dtype or fp32."""
-    return _norm_of(list(grads), max_norm, out, norm, stream)
+    return _norm_call(list(grads), max_norm, out, norm, stream)
 
 
-def _norm_of(grads, max_norm, out, norm, stream):
+def _norm_call(grads, max_norm, out, norm, stream):
     if not grads:
         raise ValueError("the list of gradients is empty")
-    outs = grads if out is None else list(out)
-    if max_norm is None:
-        table, device = _grad_list_norm(grads)
-    else:
-        table, device = _grad_list(grads, outs)
-    if norm is not None:
-        _require_one_device(grads[0], norm)
-        _check_like(norm, (), torch.float32, "norm")
-    ctx = _call_context(stream, grads[0])
+    first = grads[0]
+    ctx = _elsewhere(first, stream) if first.is_cuda else None
     if ctx is not None:
         with ctx:
-            return _norm_call(table, len(grads), max_norm, norm, device)
-    return _norm_call(table, len(grads), max_norm, norm, device)
-
-
-def _grad_list_norm(grads):
-    """As _grad_list, for reading only: a tensor may be in the list more than once."""
-    table = (capi.Grad * max(1, len(grads)))()
-    device = grads[0].device
-    for e, g in zip(table, grads):
-        _require_one_device(grads[0], g)
-        e.in_, e.n, e.dtype = g.data_ptr(), g.numel(), _dtype_code(g.dtype)
-    return table, device
-
-
-def _norm_call(table, count, max_norm, norm, device):
-    norm = torch.empty((), dtype=torch.float32, device=device) if norm is None else norm
-    need = C.c_size_t(0)
-    check(lib().cg_b200_grad_norm_workspace_bytes(count, C.byref(need)), "grad_norm_workspace_bytes")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-    if max_norm is None:
-        check(lib().cg_b200_grad_norm(table, count, _ptr(norm), _ptr(ws), need.value, _stream()), "grad_norm")
+            return _norm_call(grads, max_norm, out, norm, None)
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
+    table, words = _grad_table(grads, outs)
+    if max_norm is not None:
+        # no tensor may be written twice, and no output may be another gradient
+        pairs = [(i, o) for i, o, n in zip(words[::4], words[1::4], words[2::4]) if n]
+        written = {o for _, o in pairs}
+        if len(written) < len(pairs):
+            raise ValueError("a tensor is in the list twice")
+        if out is not None and any(i != o and i in written for i, o in pairs):
+            raise ValueError("an output is another gradient of the list")
+    if norm is None:
+        norm = torch.empty((), dtype=torch.float32, device=first.device)
     else:
-        check(lib().cg_b200_clip_grad_norm(table, count, max_norm, _ptr(norm), _ptr(ws), need.value, _stream()), "clip_grad_norm")
+        _require_one_device(first, norm)
+        _check_like(norm, (), torch.float32, "norm")
+    need = C.c_size_t(0)
+    check(lib().cg_b200_grad_norm_workspace_bytes(len(grads), C.byref(need)), "grad_norm_workspace_bytes")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=first.device)
+    grad_p, at = C.cast(table, C.POINTER(capi.Grad)), _raw_stream(first.get_device())
+    if max_norm is None:
+        check(lib().cg_b200_grad_norm(grad_p, len(grads), norm.data_ptr(), ws.data_ptr(), need.value, at), "grad_norm")
+    else:
+        check(lib().cg_b200_clip_grad_norm(grad_p, len(grads), max_norm, norm.data_ptr(), ws.data_ptr(), need.value, at),
+              "clip_grad_norm")
     return norm
 
 
