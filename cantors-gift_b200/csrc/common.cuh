@@ -75,6 +75,35 @@ __device__ __forceinline__ void peer_flag_exchange(unsigned long long* const* fl
     }
 }
 
+// ---- programmatic dependent launch ------------------------------------------------------------------
+// A kernel started by launch_pdl may begin before the kernel in front of it on the stream has ended; pdl_wait returns when that one has
+// ended and its writes are visible, so everything that depends on it comes after. pdl_trigger lets the kernel behind this one begin.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// ---- asynchronous copies into shared memory -----------------------------------------------------------
+__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most N of this thread's groups are under way
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // ---- device-side element conversion -----------------------------------------------------------
 template <typename T> struct Elem;
 template <> struct Elem<float> {

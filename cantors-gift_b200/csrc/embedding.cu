@@ -7,11 +7,10 @@
 //
 // Both are HBM-bound. Forward moves the rows that occur (L2 serves repeats) and the output. Backward reads dout once and writes the table
 // once. It sorts the (id, n) pairs by id - a stable radix sort, so equal ids stay in the order of n and the sums do not depend on
-// timing - and walks the sorted list in chunks of 32 pairs: a warp adds the rows of its chunk for 512 bytes of columns in fp32
-// registers and writes each table row that lies wholly inside the chunk. Sums of ids that reach over a chunk's edge go to the workspace
-// and a second kernel joins them in order; the table rows that no id names are zeroed beside the sums.
-#include <math.h>
-
+// timing - and walks the sorted list in chunks of 32 pairs. A warp takes a chunk for 512 bytes of columns: it adds the rows of every id
+// that begins in the chunk, in fp32 registers, following the last one into the next chunk, and writes the id's table row. Only an id
+// whose pairs cover a whole chunk and reach beyond it is added by several warps: their sums go to the workspace and a last kernel joins
+// them in order. The table rows that no id names are zeroed beside the sums.
 #include "common.cuh"
 
 namespace cgb {
@@ -115,6 +114,7 @@ struct SortParams {
     uint32_t* pos_out;
     uint32_t* count;        // [tiles][bins] of this pass
     uint32_t* count_next;   // of the next pass, or null
+    uint32_t* joins;        // length of the list of joins, cleared
     long long n, vocab, padding;
     int tiles, bins, shift, shift_next;
 };
@@ -125,13 +125,15 @@ __device__ __forceinline__ uint32_t sort_key(const SortParams& p, long long i) {
     return id < 0 || id >= p.vocab || id == p.padding ? (uint32_t)p.vocab : (uint32_t)id;
 }
 
-// First pass only: the tile's digit counts, and a cleared table for the next pass.
+// First pass only: the tile's digit counts, and cleared counts for the next pass and for the list of joins.
 template <typename I>
 __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const __grid_constant__ SortParams p) {
     __shared__ uint32_t hist[kSortBins];
+    pdl_trigger();
     for (int b = threadIdx.x; b < p.bins; b += blockDim.x) hist[b] = 0;
     __syncthreads();
     const long long base = (long long)blockIdx.x * kSortTile;
+    pdl_wait();
     for (int i = threadIdx.x; i < kSortTile; i += blockDim.x)
         if (base + i < p.n) atomicAdd(&hist[(sort_key<I>(p, base + i) >> p.shift) & (p.bins - 1)], 1u);
     __syncthreads();
@@ -139,6 +141,30 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const __gri
         p.count[(long long)blockIdx.x * p.bins + b] = hist[b];
         if (p.count_next) p.count_next[(long long)blockIdx.x * p.bins + b] = 0;
     }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.joins = 0;
+}
+
+// Inclusive scan over a warp
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// A warp's pairs of one round of 32: their ranks among the equal digits of this warp so far, counted in `cnt` (one counter per bin).
+template <typename C>
+__device__ __forceinline__ uint32_t sort_rank(C* cnt, uint32_t digit, bool live, int lane) {
+    const unsigned peers = __match_any_sync(0xffffffffu, live ? digit : 0xffffffffu);
+    const int below = __popc(peers & ((1u << lane) - 1u));
+    uint32_t before = 0;
+    if (live) before = cnt[digit];
+    __syncwarp();
+    if (live && below == 0) cnt[digit] = (C)(before + __popc(peers));
+    __syncwarp();
+    return before + below;
 }
 
 // One pass: ranks within the tile, the tile's place in every bin from the counts of all tiles, the scatter, and the next pass's counts.
@@ -148,8 +174,10 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_scatter_kernel(const __g
     __shared__ uint32_t base[kSortBins];
     __shared__ uint32_t warp_total[kSortWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_trigger();
     for (int b = threadIdx.x; b < p.bins * kSortWarps; b += blockDim.x) cnt[b / p.bins][b % p.bins] = 0;
     __syncthreads();
+    pdl_wait();
     const long long first = (long long)blockIdx.x * kSortTile + warp * (32 * kSortRounds);
     uint32_t key[kSortRounds], pos[kSortRounds], rank[kSortRounds];
 #pragma unroll
@@ -162,22 +190,23 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_scatter_kernel(const __g
             pos[r] = FIRST ? (uint32_t)i : p.pos_in[i];
         }
     }
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-        const bool live = first + r * 32 + lane < p.n;
-        const uint32_t digit = live ? (key[r] >> p.shift) & (p.bins - 1) : 0xffffffffu;
-        const unsigned peers = __match_any_sync(0xffffffffu, digit);
-        const int below = __popc(peers & ((1u << lane) - 1u));
-        uint32_t before = 0;
-        if (live) before = cnt[warp][digit];
-        __syncwarp();
-        if (live && below == 0) cnt[warp][digit] = before + __popc(peers);
-        __syncwarp();
-        rank[r] = before + below;
-    }
-    __syncthreads();
-    // thread b: bin b. Where the tile's pairs of this bin start: all pairs of lower bins, then this bin's pairs of earlier tiles.
+    // thread b: bin b's pairs in all tiles and in earlier ones
     uint32_t total = 0, earlier = 0;
+    if (threadIdx.x < p.bins) {
+#pragma unroll 16
+        for (int t = 0; t < p.tiles; ++t) {
+            const uint32_t c = p.count[(long long)t * p.bins + threadIdx.x];
+            total += c;
+            if (t < blockIdx.x) earlier += c;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+        rank[r] = sort_rank(cnt[warp], (key[r] >> p.shift) & (p.bins - 1), first + r * 32 + lane < p.n, lane);
+    const uint32_t scan = warp_scan(total, lane);
+    if (lane == 31) warp_total[warp] = scan;
+    __syncthreads();
+    // where the tile's pairs of this bin start: all pairs of lower bins, then this bin's pairs of earlier tiles
     if (threadIdx.x < p.bins) {
         uint32_t run = 0;
 #pragma unroll
@@ -186,35 +215,104 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_scatter_kernel(const __g
             cnt[w][threadIdx.x] = run;
             run += c;
         }
-#pragma unroll 8
-        for (int t = 0; t < p.tiles; ++t) {
-            const uint32_t c = p.count[(long long)t * p.bins + threadIdx.x];
-            total += c;
-            if (t < blockIdx.x) earlier += c;
-        }
+        uint32_t lower = 0;
+        for (int w = 0; w < warp; ++w) lower += warp_total[w];
+        base[threadIdx.x] = lower + scan - total + earlier;
     }
-    uint32_t scan = total;   // inclusive over the bins
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += t;
-    }
-    if (lane == 31) warp_total[warp] = scan;
-    __syncthreads();
-    uint32_t lower = 0;
-    for (int w = 0; w < warp; ++w) lower += warp_total[w];
-    if (threadIdx.x < p.bins) base[threadIdx.x] = lower + scan - total + earlier;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
-        if (first + r * 32 + lane < p.n) {
-            const uint32_t digit = (key[r] >> p.shift) & (p.bins - 1);
-            const uint32_t to = base[digit] + cnt[warp][digit] + rank[r];
+        const bool live = first + r * 32 + lane < p.n;
+        const uint32_t digit = (key[r] >> p.shift) & (p.bins - 1);
+        uint32_t to = 0;
+        if (live) {
+            to = base[digit] + cnt[warp][digit] + rank[r];
             p.key_out[to] = key[r];
             p.pos_out[to] = pos[r];
-            if (p.count_next) atomicAdd(&p.count_next[(long long)(to / kSortTile) * p.bins + ((key[r] >> p.shift_next) & (p.bins - 1))], 1u);
+        }
+        if (p.count_next) {
+            // frequent ids share a counter: one addition per warp and counter
+            const uint32_t at = live ? (to / kSortTile) * p.bins + ((key[r] >> p.shift_next) & (p.bins - 1)) : 0xffffffffu;
+            const unsigned peers = __match_any_sync(0xffffffffu, at);
+            if (live && lane == __ffs(peers) - 1) atomicAdd(&p.count_next[at], (uint32_t)__popc(peers));
         }
     }
+}
+
+// Up to kSortSmall pairs in one CTA: every pass through shared memory, one launch instead of one per pass and one for the counts.
+constexpr int kSortSmall = 8192, kSmallWarps = 32, kSmallRounds = kSortSmall / (32 * kSmallWarps);
+struct SortSmall {
+    uint32_t key[kSortSmall];
+    uint16_t pos[kSortSmall];
+    uint16_t cnt[kSmallWarps][kSortBins];
+    uint32_t base[kSortBins];
+    uint32_t warp_total[kSmallWarps];
+};
+template <typename I>
+__global__ void __launch_bounds__(kSmallWarps * 32) sort_small_kernel(const __grid_constant__ SortParams p, int passes, int digit_bits) {
+    extern __shared__ float4 sort_smem4[];
+    SortSmall& sm = *reinterpret_cast<SortSmall*>(sort_smem4);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (int)p.n;
+    // the warps share the pairs evenly, in whole rounds
+    const int rounds = (n + 32 * kSmallWarps - 1) / (32 * kSmallWarps), first = warp * rounds * 32 + lane;
+    pdl_trigger();
+    uint32_t key[kSmallRounds], rank[kSmallRounds];
+    uint32_t pos[kSmallRounds];
+    pdl_wait();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r) {
+        const int i = first + r * 32;
+        pos[r] = (uint32_t)i;
+        key[r] = r < rounds && i < n ? sort_key<I>(p, i) : 0xffffffffu;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * digit_bits;
+        for (int b = threadIdx.x; b < p.bins * kSmallWarps; b += blockDim.x) sm.cnt[b / p.bins][b % p.bins] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r)
+            if (r < rounds) rank[r] = sort_rank(sm.cnt[warp], (key[r] >> shift) & (p.bins - 1), first + r * 32 < n, lane);
+        __syncthreads();
+        uint32_t total = 0;
+        if (threadIdx.x < p.bins) {
+#pragma unroll
+            for (int w = 0; w < kSmallWarps; ++w) {
+                const uint32_t c = sm.cnt[w][threadIdx.x];
+                sm.cnt[w][threadIdx.x] = (uint16_t)total;
+                total += c;
+            }
+        }
+        const uint32_t scan = warp_scan(total, lane);
+        if (lane == 31) sm.warp_total[warp] = scan;
+        __syncthreads();
+        if (threadIdx.x < p.bins) {
+            uint32_t lower = 0;
+            for (int w = 0; w < warp; ++w) lower += sm.warp_total[w];
+            sm.base[threadIdx.x] = lower + scan - total;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r)
+            if (r < rounds && first + r * 32 < n) {
+                const uint32_t digit = (key[r] >> shift) & (p.bins - 1), to = sm.base[digit] + sm.cnt[warp][digit] + rank[r];
+                sm.key[to] = key[r];
+                sm.pos[to] = (uint16_t)pos[r];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r)
+            if (r < rounds && first + r * 32 < n) {
+                key[r] = sm.key[first + r * 32];
+                pos[r] = sm.pos[first + r * 32];
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r)
+        if (r < rounds && first + r * 32 < n) {
+            p.key_out[first + r * 32] = key[r];
+            p.pos_out[first + r * 32] = pos[r];
+        }
+    if (threadIdx.x == 0) *p.joins = 0;
 }
 
 // ---- sums over the sorted list ---------------------------------------------------------------------------
@@ -225,204 +323,303 @@ struct EmbGradParams {
     const uint32_t* key;   // sorted
     const uint32_t* pos;
     void* dtable;
-    float* part;           // [chunks][2][cols]: a chunk's sum of the id that reaches in from before it, of the id that reaches out behind it
+    float* part;           // [chunks][2][cols]: a chunk's sum of an id that began before it, and of one that begins in it and is joined
+    uint32_t* joins;       // how many ids are joined, and the chunks where they begin
     long long n, vocab, cols, chunks;
-    long long sum_blocks;  // blocks that add; the others zero
+    int zero_blocks;       // the first blocks zero, the others add
     float scale;
     int accumulate;
     int tiles;             // column tiles of a row
 };
 
-// W columns from c0 on of table row `row` (fewer at the row's end)
-template <typename G, int W, bool VEC>
-__device__ __forceinline__ void emb_write(const EmbGradParams& p, long long row, long long c0, const float (&acc)[W]) {
-    G* dst = static_cast<G*>(p.dtable) + row * p.cols + c0;
-    if constexpr (VEC) {
-        constexpr int M = Vec16<G>::N;   // M <= W: the table's gradient has the rows' type or fp32
+// The columns of a lane: NP pieces of E columns, 32 * E apart; E columns are one store of the table's type. Without vectors E is 1.
+template <typename G, int E, int NP>
+struct EmbLane {
+    float v[NP][E];
+    __device__ void clear() {
 #pragma unroll
-        for (int l = 0; l < W; l += M) {
-            float f[M];
+        for (int q = 0; q < NP; ++q)
 #pragma unroll
-            for (int i = 0; i < M; ++i) f[i] = acc[l + i] * p.scale;
-            if (p.accumulate) {
-                float old[M];
-                unpack16<G>(*reinterpret_cast<const Vec16<G>*>(dst + l), old);
-#pragma unroll
-                for (int i = 0; i < M; ++i) f[i] += old[i];
-            }
-            st_stream(dst + l, pack16<G>(f));
-        }
-    } else {
-#pragma unroll
-        for (int l = 0; l < W; ++l) {
-            const long long c = c0 + l * 32;
-            if (c < p.cols) {
-                float f = acc[l] * p.scale;
-                if (p.accumulate) f += Elem<G>::to_f32(dst[l * 32]);
-                dst[l * 32] = Elem<G>::from_f32(f);
-            }
-        }
+            for (int l = 0; l < E; ++l) v[q][l] = 0.0f;
     }
-}
-
-template <int W, bool VEC>
-__device__ __forceinline__ void emb_write_part(const EmbGradParams& p, long long chunk, int slot, long long c0, const float (&acc)[W]) {
-    float* dst = p.part + (chunk * 2 + slot) * p.cols + c0;
+    // into row `row` of the table's gradient
+    __device__ void write(const EmbGradParams& p, long long row, long long c0) const {
+        G* dst = static_cast<G*>(p.dtable) + row * p.cols + c0;
 #pragma unroll
-    for (int l = 0; l < W; ++l) {
-        if constexpr (VEC) {
-            if (l % 4 == 0) *reinterpret_cast<float4*>(dst + l) = make_float4(acc[l], acc[l + 1], acc[l + 2], acc[l + 3]);
-        } else if (c0 + l * 32 < p.cols) {
-            dst[l * 32] = acc[l];
-        }
-    }
-}
-
-// VEC: lane t owns the L columns of packet t of the tile; otherwise columns t, t + 32, ... (8 of them), read one by one.
-template <typename T, typename G, bool VEC>
-__global__ void __launch_bounds__(256) emb_grad_kernel(const __grid_constant__ EmbGradParams p) {
-    constexpr int W = VEC ? Vec16<T>::N : 8, U = 8;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (blockIdx.x >= p.sum_blocks) {
-        // table rows that no id names: a lane looks one row up in the sorted list, the warp zeroes those that are missing
-        const long long step = ((long long)gridDim.x - p.sum_blocks) * 8;
-        for (long long r0 = (((long long)blockIdx.x - p.sum_blocks) * 8 + warp) * 32; r0 < p.vocab; r0 += step * 32) {
-            bool missing = false;
-            if (r0 + lane < p.vocab) {
-                const uint32_t v = (uint32_t)(r0 + lane);
-                long long lo = 0, hi = p.n;
-                while (lo < hi) {
-                    const long long mid = (lo + hi) >> 1;
-                    if (__ldg(p.key + mid) < v) lo = mid + 1;
-                    else hi = mid;
-                }
-                missing = lo == p.n || __ldg(p.key + lo) != v;
-            }
-            unsigned todo = __ballot_sync(0xffffffffu, missing);
-            while (todo) {
-                const long long row = r0 + __ffs(todo) - 1;
-                todo &= todo - 1;
-                G* dst = static_cast<G*>(p.dtable) + row * p.cols;
-                if (VEC && p.cols % Vec16<G>::N == 0) {
-                    for (long long k = lane; k < p.cols / Vec16<G>::N; k += 32) __stcs(reinterpret_cast<int4*>(dst) + k, make_int4(0, 0, 0, 0));
+        for (int q = 0; q < NP; ++q)
+            if (c0 + q * 32 * E < p.cols) {
+                float f[E];
+#pragma unroll
+                for (int l = 0; l < E; ++l) f[l] = v[q][l] * p.scale;
+                if constexpr (E == 1) {
+                    if (p.accumulate) f[0] += Elem<G>::to_f32(dst[q * 32]);
+                    dst[q * 32] = Elem<G>::from_f32(f[0]);
                 } else {
-                    for (long long c = lane; c < p.cols; c += 32) dst[c] = Elem<G>::from_f32(0.0f);
+                    if (p.accumulate) {
+                        float old[E];
+                        unpack16<G>(*reinterpret_cast<const Vec16<G>*>(dst + q * 32 * E), old);
+#pragma unroll
+                        for (int l = 0; l < E; ++l) f[l] += old[l];
+                    }
+                    st_stream(dst + q * 32 * E, pack16<G>(f));
                 }
             }
-        }
-        return;
     }
-    const long long unit = (long long)blockIdx.x * 8 + warp;
+    // into the workspace
+    __device__ void write_part(const EmbGradParams& p, long long chunk, int slot, long long c0) const {
+        float* dst = p.part + (chunk * 2 + slot) * p.cols + c0;
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+            if (c0 + q * 32 * E < p.cols) {
+                if constexpr (E == 1) {
+                    dst[q * 32] = v[q][0];
+                } else {
+#pragma unroll
+                    for (int l = 0; l < E; l += 4)
+                        *reinterpret_cast<float4*>(dst + q * 32 * E + l) = make_float4(v[q][l], v[q][l + 1], v[q][l + 2], v[q][l + 3]);
+                }
+            }
+    }
+};
+
+// Table rows that no id names: a lane looks one row up in the sorted list, the warp zeroes those that are missing.
+template <typename G, bool VEC>
+__device__ __forceinline__ void emb_zero(const EmbGradParams& p, int lane, int warp) {
+    const long long step = (long long)p.zero_blocks * 8 * 32;
+    for (long long r0 = ((long long)blockIdx.x * 8 + warp) * 32; r0 < p.vocab; r0 += step) {
+        bool missing = false;
+        if (r0 + lane < p.vocab) {
+            const uint32_t v = (uint32_t)(r0 + lane);
+            long long lo = 0, hi = p.n;
+            while (lo < hi) {
+                const long long mid = (lo + hi) >> 1;
+                if (p.key[mid] < v) lo = mid + 1;
+                else hi = mid;
+            }
+            missing = lo == p.n || p.key[lo] != v;
+        }
+        unsigned todo = __ballot_sync(0xffffffffu, missing);
+        while (todo) {
+            const long long row = r0 + __ffs(todo) - 1;
+            todo &= todo - 1;
+            G* dst = static_cast<G*>(p.dtable) + row * p.cols;
+            if constexpr (VEC) {
+                for (long long k = lane; k < p.cols / Vec16<G>::N; k += 32) __stcs(reinterpret_cast<int4*>(dst) + k, make_int4(0, 0, 0, 0));
+            } else {
+                for (long long c = lane; c < p.cols; c += 32) dst[c] = Elem<G>::from_f32(0.0f);
+            }
+        }
+    }
+}
+
+// What a warp does with its chunk: the pairs begin .. end - 1 of this chunk and the next one's are its own.
+struct EmbSpan {
+    uint32_t key, pos, key2, pos2;   // lane l's pair of this chunk and of the next
+    int begin, end;
+    int slot;        // where the sum of the last id goes: -1 the table, 0 / 1 the workspace
+    bool head_part;  // the first id's sum goes to the workspace (and it is not the last id)
+    __device__ uint32_t id(int i) const { return __shfl_sync(0xffffffffu, i < kChunk ? key : key2, i & 31); }
+    __device__ uint32_t at(int i) const { return __shfl_sync(0xffffffffu, i < kChunk ? pos : pos2, i & 31); }
+};
+__device__ __forceinline__ EmbSpan emb_span(const EmbGradParams& p, long long chunk, int lane) {
+    const long long first = chunk * kChunk;
+    const uint32_t none = (uint32_t)p.vocab;
+    const bool here = first + lane < p.n, there = first + kChunk + lane < p.n;
+    EmbSpan s;
+    s.key = here ? p.key[first + lane] : none;
+    s.pos = here ? p.pos[first + lane] : 0;
+    s.key2 = there ? p.key[first + kChunk + lane] : none;
+    s.pos2 = there ? p.pos[first + kChunk + lane] : 0;
+    const uint32_t before = first > 0 ? p.key[first - 1] : none, before32 = first > 0 ? p.key[first - kChunk] : none;
+    const uint32_t id0 = __shfl_sync(0xffffffffu, s.key, 0), id31 = __shfl_sync(0xffffffffu, s.key, 31);
+    const uint32_t id32 = __shfl_sync(0xffffffffu, s.key2, 0), id63 = __shfl_sync(0xffffffffu, s.key2, 31);
+    s.begin = 0;
+    s.end = __popc(__ballot_sync(0xffffffffu, s.key != none));   // dropped ids are last
+    s.slot = -1;
+    s.head_part = false;
+    const bool full = id0 == id31 && id0 != none, head = id0 == before && id0 != none;
+    if (head && !full) {
+        const int same = __popc(__ballot_sync(0xffffffffu, s.key == id0));
+        if (before32 == id0) s.head_part = true;   // joined
+        else s.begin = same;                        // the warp of the chunk before adds it
+    }
+    if (full && head) {
+        s.slot = 0;
+    } else if (id31 != none && id32 == id31) {      // the last id goes on
+        const int more = __popc(__ballot_sync(0xffffffffu, s.key2 == id31));
+        if (full || id63 == id31) s.slot = 1;
+        else s.end += more;                         // into the next chunk, to its end
+    }
+    return s;
+}
+
+// The rows come through shared memory, sixteen of a warp's 512-byte pieces under way at a time: requested as register loads they would
+// either cost the registers of as many packets or be waited for one by one (86 us instead of {GRAD_US} us for 57344 rows of 1024 bf16).
+constexpr int kEmbRows = 4, kEmbGroups = 4;   // rows of a copy group, groups in flight
+template <typename T, typename G>
+__global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant__ EmbGradParams p) {
+    constexpr int L = Vec16<T>::N, E = Vec16<G>::N < L ? Vec16<G>::N : L, NP = L / E;
+    extern __shared__ float4 emb_smem4[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.x < p.zero_blocks) return emb_zero<G, true>(p, lane, warp);
+    const long long unit = (long long)(blockIdx.x - p.zero_blocks) * 8 + warp;
     const long long chunk = unit / p.tiles;
     if (chunk >= p.chunks) return;
-    const long long c0 = (unit - chunk * p.tiles) * (32 * W) + (VEC ? lane * W : lane);
-    const bool in = c0 < p.cols;
-    const long long first = chunk * kChunk;
-    const int count = (int)(p.n - first < kChunk ? p.n - first : kChunk);
-    const uint32_t none = (uint32_t)p.vocab;
-    const uint32_t key = lane < count ? p.key[first + lane] : none;
-    const uint32_t pos = lane < count ? p.pos[first + lane] : 0;
-    const uint32_t before = first > 0 ? p.key[first - 1] : none;
-    const uint32_t behind = first + count < p.n ? p.key[first + count] : none;
-    const T* dout = static_cast<const T*>(p.dout);
-    float acc[W];
+    const long long tile0 = (unit - chunk * p.tiles) * (32 * L), c0 = tile0 + lane * E;
+    const EmbSpan span = emb_span(p, chunk, lane);
+    if (span.begin >= span.end) return;
+    if (span.slot == 1 && tile0 == 0 && lane == 0) p.joins[1 + atomicAdd(p.joins, 1u)] = (uint32_t)chunk;   // in any order: each is joined by itself
+    // a warp's ring: [groups][rows][32 packets]; lane l copies packet l of a row and reads the pieces of its own columns
+    Vec16<T>* ring = reinterpret_cast<Vec16<T>*>(emb_smem4) + warp * (kEmbGroups * kEmbRows * 32);
+    const T* src = static_cast<const T*>(p.dout) + tile0 + lane * L;
+    const bool in = tile0 + lane * L < p.cols;   // whole packets: cols is a multiple of L
+    auto fetch = [&](int group, int i) {   // rows i .. of the span into group `group`
 #pragma unroll
-    for (int l = 0; l < W; ++l) acc[l] = 0.0f;
-    uint32_t cur = __shfl_sync(0xffffffffu, key, 0);
-    bool head = cur == before;   // the current id began in an earlier chunk
-    if (cur == none) return;     // dropped ids are last: nothing here
-    for (int i0 = 0; i0 < count; i0 += U) {
-        Vec16<T> raw[U];
-        float one[VEC ? 1 : U][VEC ? 1 : W];
+        for (int r = 0; r < kEmbRows; ++r)
+            if (i + r < span.end) {
+                const T* from = src + (long long)span.at(i + r) * p.cols;
+                if (in) copy16_async(ring + (group * kEmbRows + r) * 32 + lane, from);
+            }
+        copy_commit();
+    };
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t k = __shfl_sync(0xffffffffu, key, i0 + u);
-            const T* src = dout + (long long)__shfl_sync(0xffffffffu, pos, i0 + u) * p.cols + c0;
-            if (k != none && in) {
-                if constexpr (VEC) {
-                    raw[u] = ld_stream(src);
-                } else {
+    for (int g = 0; g < kEmbGroups; ++g) fetch(g, span.begin + g * kEmbRows);
+    EmbLane<G, E, NP> acc;
+    acc.clear();
+    uint32_t cur = span.id(span.begin);
+    bool head_part = span.head_part;
+    int group = 0;
+    for (int i0 = span.begin; i0 < span.end; i0 += kEmbRows) {
+        copy_wait<kEmbGroups - 1>();
+        __syncwarp();
 #pragma unroll
-                    for (int l = 0; l < W; ++l) one[u][l] = c0 + l * 32 < p.cols ? Elem<T>::to_f32(src[l * 32]) : 0.0f;
-                }
+        for (int r = 0; r < kEmbRows; ++r) {
+            if (i0 + r >= span.end) break;
+            const uint32_t id = span.id(i0 + r);
+            if (id != cur) {
+                if (head_part) acc.write_part(p, chunk, 0, c0);
+                else acc.write(p, cur, c0);
+                head_part = false;
+                cur = id;
+                acc.clear();
+            }
+            const T* row = reinterpret_cast<const T*>(ring + (group * kEmbRows + r) * 32);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                Vec16<T> v;
+                if constexpr (NP == 1) v = *reinterpret_cast<const Vec16<T>*>(row + lane * E);
+                else *reinterpret_cast<int2*>(&v) = *reinterpret_cast<const int2*>(row + q * 32 * E + lane * E);   // half a packet
+                float t[L];
+                unpack16<T>(v, t);
+#pragma unroll
+                for (int l = 0; l < E; ++l) acc.v[q][l] += t[l];
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t k = __shfl_sync(0xffffffffu, key, i0 + u);
-            if (k != cur && cur != none) {
-                if (in) {
-                    if (head) emb_write_part<W, VEC>(p, chunk, 0, c0, acc);
-                    else emb_write<G, W, VEC>(p, cur, c0, acc);
-                }
-                head = false;
-                cur = k;
-#pragma unroll
-                for (int l = 0; l < W; ++l) acc[l] = 0.0f;
-            }
-            if (k != none && in) {
-                float f[W];
-                if constexpr (VEC) {
-                    unpack16<T>(raw[u], f);
-                } else {
-#pragma unroll
-                    for (int l = 0; l < W; ++l) f[l] = one[u][l];
-                }
-#pragma unroll
-                for (int l = 0; l < W; ++l) acc[l] += f[l];
-            }
-        }
+        __syncwarp();
+        fetch(group, i0 + kEmbGroups * kEmbRows);
+        group = group + 1 == kEmbGroups ? 0 : group + 1;
     }
-    if (cur != none && in) {
-        if (head) emb_write_part<W, VEC>(p, chunk, 0, c0, acc);
-        else if (cur == behind) emb_write_part<W, VEC>(p, chunk, 1, c0, acc);
-        else emb_write<G, W, VEC>(p, cur, c0, acc);
-    }
+    if (head_part) acc.write_part(p, chunk, 0, c0);
+    else if (span.slot >= 0) acc.write_part(p, chunk, span.slot, c0);
+    else acc.write(p, cur, c0);
 }
 
-// Joins an id's sums over the chunks it reaches across. A CTA per chunk and share of the columns; only the chunk where an id begins that
-// reaches beyond it has work. A few sums are added by the warp that owns the columns, many by all eight warps of the CTA, each every
-// eighth sum: the split depends on the number of sums alone.
-template <typename G>
-__global__ void __launch_bounds__(256) emb_join_kernel(const __grid_constant__ EmbGradParams p) {
-    __shared__ float sum[8][32];
-    const long long chunk = blockIdx.x, first = chunk * kChunk, end = first + kChunk;
-    if (end >= p.n) return;
-    const uint32_t none = (uint32_t)p.vocab, id = p.key[end - 1];
-    if (id == none || p.key[end] != id) return;                             // nothing reaches out of this chunk
-    if (p.key[first] == id && first > 0 && p.key[first - 1] == id) return;    // it began earlier
+// Any width and alignment: a lane owns eight columns, 32 apart, and reads them one by one.
+template <typename T, typename G>
+__global__ void __launch_bounds__(256) emb_grad_scalar_kernel(const __grid_constant__ EmbGradParams p) {
+    constexpr int NP = 8, U = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // the chunk with the id's last pair: chunk `last` begins with a pair of the id, chunk `hi` does not; 32 probes per step
-    long long last = chunk + 1, hi = p.chunks;
-    while (hi - last > 1) {
-        const long long span = (hi - last + 31) / 32, at = last + span * (lane + 1);
-        const int passed = __popc(__ballot_sync(0xffffffffu, at < hi && p.key[at * kChunk] == id));
-        const long long beyond = last + span * (passed + 1);
-        last += span * passed;
-        if (beyond < hi) hi = beyond;
-    }
-    const bool together = last - chunk > 16;
-    const int from = together ? warp : 0, step = together ? 8 : 1;
-    const long long tiles = (p.cols + 31) / 32;
-    for (long long t = together ? blockIdx.y : (long long)blockIdx.y * 8 + warp; t < tiles; t += (long long)gridDim.y * (together ? 1 : 8)) {
-        const long long c = t * 32 + lane;
-        float s = 0.0f;
-        if (c < p.cols) {
-            if (from == 0) s = p.part[(chunk * 2 + 1) * p.cols + c];
-#pragma unroll 8
-            for (long long k = chunk + 1 + from; k <= last; k += step) s += p.part[k * 2 * p.cols + c];
-        }
-        if (together) {
-            __syncthreads();
-            sum[warp][lane] = s;
-            __syncthreads();
-            if (warp != 0) continue;
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.x < p.zero_blocks) return emb_zero<G, false>(p, lane, warp);
+    const long long unit = (long long)(blockIdx.x - p.zero_blocks) * 8 + warp;
+    const long long chunk = unit / p.tiles;
+    if (chunk >= p.chunks) return;
+    const long long c0 = (unit - chunk * p.tiles) * (32 * NP) + lane;
+    const EmbSpan span = emb_span(p, chunk, lane);
+    if (span.begin >= span.end) return;
+    if (span.slot == 1 && c0 == 0) p.joins[1 + atomicAdd(p.joins, 1u)] = (uint32_t)chunk;
+    EmbLane<G, 1, NP> acc;
+    acc.clear();
+    uint32_t cur = span.id(span.begin);
+    bool head_part = span.head_part;
+    for (int i0 = span.begin; i0 < span.end; i0 += U) {
+        float v[U][NP];
 #pragma unroll
-            for (int w = 1; w < 8; ++w) s += sum[w][lane];
+        for (int u = 0; u < U; ++u) {
+            const T* src = static_cast<const T*>(p.dout) + (long long)span.at(i0 + u) * p.cols + c0;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) v[u][q] = i0 + u < span.end && c0 + q * 32 < p.cols ? Elem<T>::to_f32(src[q * 32]) : 0.0f;
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= span.end) break;
+            const uint32_t id = span.id(i0 + u);
+            if (id != cur) {
+                if (head_part) acc.write_part(p, chunk, 0, c0);
+                else acc.write(p, cur, c0);
+                head_part = false;
+                cur = id;
+                acc.clear();
+            }
+#pragma unroll
+            for (int q = 0; q < NP; ++q) acc.v[q][0] += v[u][q];
+        }
+    }
+    if (head_part) acc.write_part(p, chunk, 0, c0);
+    else if (span.slot >= 0) acc.write_part(p, chunk, span.slot, c0);
+    else acc.write(p, cur, c0);
+}
+
+// Joins the sums of an id over the chunks that it covers: a CTA per id and 32 * E columns, sixteen strands of sums, each in order.
+template <typename G, int E>
+__global__ void __launch_bounds__(512) emb_join_kernel(const __grid_constant__ EmbGradParams p) {
+    __shared__ float sum[16][32 * E + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_trigger();
+    pdl_wait();
+    const long long tiles = (p.cols + 32 * E - 1) / (32 * E), units = (long long)p.joins[0] * tiles;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+        const long long chunk = p.joins[1 + u / tiles], c = u % tiles * (32 * E) + lane * E;
+        const uint32_t id = p.key[chunk * kChunk + kChunk - 1];
+        // the chunk with the id's last pair: chunk `last` begins with a pair of the id, chunk `hi` does not; 32 probes per step
+        long long last = chunk + 1, hi = p.chunks;
+        for (long long span = 1; hi - last > 1; span = (hi - last + 31) / 32) {   // the next 32 chunks first, where most ids end
+            const long long at = last + span * (lane + 1);
+            const int passed = __popc(__ballot_sync(0xffffffffu, at < hi && p.key[at * kChunk] == id));
+            const long long beyond = last + span * (passed + 1);
+            last += span * passed;
+            if (passed < 32 && beyond < hi) hi = beyond;
+        }
+        float s[E];
+#pragma unroll
+        for (int l = 0; l < E; ++l) s[l] = 0.0f;
+        auto add = [&](const float* from) {
+            if constexpr (E == 4) {
+                const float4 t = *reinterpret_cast<const float4*>(from);
+                s[0] += t.x; s[1] += t.y; s[2] += t.z; s[3] += t.w;
+            } else {
+                s[0] += *from;
+            }
+        };
         if (c < p.cols) {
-            G* dst = static_cast<G*>(p.dtable) + (long long)id * p.cols + c;
-            float f = s * p.scale;
+            if (warp == 0) add(p.part + (chunk * 2 + 1) * p.cols + c);
+#pragma unroll 8
+            for (long long k = chunk + 1 + warp; k <= last; k += 16) add(p.part + k * 2 * p.cols + c);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int l = 0; l < E; ++l) sum[warp][lane * E + l] = s[l];
+        __syncthreads();
+        const long long cc = u % tiles * (32 * E) + threadIdx.x;
+        if (threadIdx.x < 32 * E && cc < p.cols) {
+            float f = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) f += sum[w][threadIdx.x];
+            G* dst = static_cast<G*>(p.dtable) + (long long)id * p.cols + cc;
+            f *= p.scale;
             if (p.accumulate) f += Elem<G>::to_f32(*dst);
             *dst = Elem<G>::from_f32(f);
         }
@@ -431,7 +628,7 @@ __global__ void __launch_bounds__(256) emb_join_kernel(const __grid_constant__ E
 
 // Parts of the workspace, each 256-byte aligned
 struct EmbWorkspace {
-    size_t key[2], pos[2], count[2], part, bytes;
+    size_t key[2], pos[2], count[2], joins, part, bytes;
     long long chunks;
     int tiles, passes, digit_bits;
 };
@@ -455,6 +652,7 @@ static EmbWorkspace emb_workspace(long long n, long long vocab, long long cols) 
         w.pos[i] = take((size_t)n * 4);
         w.count[i] = take(((size_t)w.tiles << w.digit_bits) * 4);
     }
+    w.joins = take((size_t)(w.chunks + 1) * 4);
     w.part = take((size_t)w.chunks * 2 * (size_t)cols * 4);
     w.bytes = at;
     return w;
@@ -469,6 +667,16 @@ static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long 
     p.padding = padding;
     p.tiles = w.tiles;
     p.bins = 1 << w.digit_bits;
+    p.joins = reinterpret_cast<uint32_t*>(ws + w.joins);
+    if (n <= kSortSmall) {
+        p.key_out = reinterpret_cast<uint32_t*>(ws + w.key[0]);
+        p.pos_out = reinterpret_cast<uint32_t*>(ws + w.pos[0]);
+        CGB_CUDA(cudaFuncSetAttribute(sort_small_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmall)));
+        sort_small_kernel<I><<<1, kSmallWarps * 32, sizeof(SortSmall), s>>>(p, w.passes, w.digit_bits);
+        CGB_CUDA(cudaGetLastError());
+        *result = 0;
+        return CG_B200_OK;
+    }
     int cur = 0;
     for (int pass = 0; pass < w.passes; ++pass) {
         p.shift = pass * w.digit_bits;
@@ -481,10 +689,12 @@ static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long 
         p.pos_out = reinterpret_cast<uint32_t*>(ws + w.pos[cur ^ 1]);
         if (pass == 0) {
             sort_count_kernel<I><<<w.tiles, kSortWarps * 32, 0, s>>>(p);
-            sort_scatter_kernel<I, true><<<w.tiles, kSortWarps * 32, 0, s>>>(p);
-        } else {
-            if (p.count_next) CGB_CUDA(cudaMemsetAsync(p.count_next, 0, ((size_t)w.tiles << w.digit_bits) * 4, s));
+            CGB_CUDA(launch_pdl(sort_scatter_kernel<I, true>, w.tiles, kSortWarps * 32, 0, s, p));
+        } else if (p.count_next) {
+            CGB_CUDA(cudaMemsetAsync(p.count_next, 0, ((size_t)w.tiles << w.digit_bits) * 4, s));
             sort_scatter_kernel<I, false><<<w.tiles, kSortWarps * 32, 0, s>>>(p);
+        } else {
+            CGB_CUDA(launch_pdl(sort_scatter_kernel<I, false>, w.tiles, kSortWarps * 32, 0, s, p));
         }
         CGB_CUDA(cudaGetLastError());
         cur ^= 1;
@@ -495,21 +705,25 @@ static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long 
 
 template <typename T, typename G>
 static int emb_backward(EmbGradParams p, cudaStream_t s) {
-    const bool vec = p.cols % Vec16<T>::N == 0 && p.cols % Vec16<G>::N == 0 && aligned_to(p.dout, 16) && aligned_to(p.dtable, 16);
-    const long long per = vec ? 32 * Vec16<T>::N : 256;
+    constexpr int L = Vec16<T>::N;
+    const bool vec = p.cols % L == 0 && aligned_to(p.dout, 16) && aligned_to(p.dtable, 16);
+    const long long per = vec ? 32 * L : 256;
     p.tiles = (int)((p.cols + per - 1) / per);
-    p.sum_blocks = (p.chunks * p.tiles + 7) / 8;
     const long long zero_cap = (long long)sm_count() * 8, want = (p.vocab + 255) / 256;
-    const long long blocks = p.sum_blocks + (p.accumulate ? 0 : want < zero_cap ? want : zero_cap);
+    p.zero_blocks = p.accumulate ? 0 : (int)(want < zero_cap ? want : zero_cap);
+    const long long blocks = (p.chunks * p.tiles + 7) / 8 + p.zero_blocks;
     if (blocks > 0x7fffffffll) return CG_B200_ERR_UNSUPPORTED;
-    if (blocks > 0) {
-        if (vec) emb_grad_kernel<T, G, true><<<(unsigned)blocks, 256, 0, s>>>(p);
-        else emb_grad_kernel<T, G, false><<<(unsigned)blocks, 256, 0, s>>>(p);
-        CGB_CUDA(cudaGetLastError());
+    if (vec) {
+        constexpr int smem = 8 * kEmbGroups * kEmbRows * 512;
+        CGB_CUDA(cudaFuncSetAttribute(emb_grad_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CGB_CUDA(launch_pdl(emb_grad_kernel<T, G>, (unsigned)blocks, 256, smem, s, p));
+    } else {
+        CGB_CUDA(launch_pdl(emb_grad_scalar_kernel<T, G>, (unsigned)blocks, 256, 0, s, p));
     }
-    if (p.chunks > 1) {
-        emb_join_kernel<G><<<dim3((unsigned)p.chunks, p.cols > 256 ? 4 : 1), 256, 0, s>>>(p);
-        CGB_CUDA(cudaGetLastError());
+    if (p.n > kChunk) {   // fewer cannot cover a chunk and reach beyond it
+        const int e = p.cols % 4 == 0 ? 4 : 1;
+        const long long units = p.chunks * ((p.cols + 32 * e - 1) / (32 * e)), cap = (long long)sm_count() * 4;
+        CGB_CUDA(launch_pdl(e == 4 ? emb_join_kernel<G, 4> : emb_join_kernel<G, 1>, (unsigned)(units < cap ? units : cap), 512, 0, s, p));
     }
     return CG_B200_OK;
 }
@@ -586,6 +800,7 @@ extern "C" int cg_b200_embedding_backward(int dtype, int grad_dtype, const void*
     p.pos = reinterpret_cast<const uint32_t*>(ws + w.pos[sorted]);
     p.dtable = dtable;
     p.part = reinterpret_cast<float*>(ws + w.part);
+    p.joins = reinterpret_cast<uint32_t*>(ws + w.joins);
     p.n = n;
     p.vocab = vocab;
     p.cols = cols;

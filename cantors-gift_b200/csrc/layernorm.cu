@@ -87,15 +87,11 @@ __device__ __forceinline__ void row_sum(LnSums<N>& s, LnSums<N>* scratch, int& p
     }
 }
 
-__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // until at most `stages` - 1 of this thread's groups are under way
-__device__ __forceinline__ void copy_wait(int stages) {
-    if (stages >= 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+__device__ __forceinline__ void ln_wait(int stages) {
+    if (stages >= 3) copy_wait<2>();
+    else if (stages == 2) copy_wait<1>();
+    else copy_wait<0>();
 }
 
 // Where a ragged row's ends lie: `head` columns of packet 0 and all from `tail` on in packet `last` belong to its neighbours. A CTA's rows
@@ -274,7 +270,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
     for (int i = 0; i < left; i += R) {
         Vec16<T>* slot = ring + stage * R * CH * kLnThreads;
         stage = stage + 1 == sh.stages ? 0 : stage + 1;
-        copy_wait(sh.stages);
+        ln_wait(sh.stages);
         float2 x[R][CH][L / 2];
         LnSums<R> s;
 #pragma unroll
@@ -439,7 +435,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
             rstd[r] = rstd_n[r];
         }
         statistics(i + R);
-        copy_wait(sh.stages);
+        ln_wait(sh.stages);
         constexpr int K = KEEP ? CH : 1;   // packets held at a time
         float2 h[R][K][L / 2], t[R][K][L / 2];
         // x and dy of packets j0 .. j0 + K - 1 of row r, into h and t
@@ -533,7 +529,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
     }
     if (!p.part) return;
     // this CTA's sums: the groups' registers are added in the order of the groups
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    copy_wait<0>();
     float* sum = reinterpret_cast<float*>(ln_smem4);
     float* part = p.part + (long long)blockIdx.x * 2 * p.cols;
     const int span = tpr * CH * L;   // the columns a group covers
