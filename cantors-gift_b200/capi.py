@@ -123,8 +123,8 @@ SIGNATURES = {
     "cg_b200_embedding_backward_workspace_bytes": (_i, [_i64, _i64, _i64, C.POINTER(_sz)]),
     "cg_b200_embedding_backward": (_i, [_i, _i, _vp, _vp, _i, _i64, C.c_float, _i64, _i, _vp, _i64, _i64, _vp, _sz, _vp]),
     "cg_b200_grad_norm_workspace_bytes": (_i, [_i64, C.POINTER(_sz)]),
-    "cg_b200_grad_norm": (_i, [C.POINTER(Grad), _i64, _vp, _vp, _sz, _vp]),
-    "cg_b200_clip_grad_norm": (_i, [C.POINTER(Grad), _i64, C.c_float, _vp, _vp, _sz, _vp]),
+    "cg_b200_grad_norm": (_i, [_vp, _i64, _vp, _vp, _sz, _vp]),
+    "cg_b200_clip_grad_norm": (_i, [_vp, _i64, C.c_float, _vp, _vp, _sz, _vp]),
     "cg_b200_attention": (_i, [C.POINTER(AttentionDesc), _vp, _vp, _vp, _vp, _vp]),
     "cg_b200_gemm_workspace_bytes": (_i, [C.POINTER(GemmDesc), C.POINTER(_sz)]),
     "cg_b200_gemm": (_i, [C.POINTER(GemmDesc), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

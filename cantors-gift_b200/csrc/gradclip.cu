@@ -6,18 +6,23 @@
 //
 // HBM-bound: the list is read for the norm and again for the scaling, which cannot begin before the norm is known, and written once.
 // The tensors' addresses, lengths and types travel by value in the kernel's parameters, so nothing is copied to the device first and
-// nothing is kept between calls. Each tensor is cut into chunks of 16384 elements and the CTAs walk the chunks of all tensors
-// gridDim.x apart; squares are added in fp32 per 16-byte packet and in fp64 beyond it, and every CTA leaves one fp64 sum in the
+// nothing is kept between calls. Each tensor is cut into chunks and the CTAs walk the chunks of all tensors gridDim.x apart; squares are added in fp32 per 16-byte packet and in fp64 beyond it, and every CTA leaves one fp64 sum in the
 // workspace. The scaling kernel's CTAs each add those sums up in the same fixed order, so the norm does not depend on timing, and walk
-// the chunks backwards: what the norm pass read last is still in L2.
+// their pieces backwards: what the norm pass read last is still in L2.
 #include <float.h>
+#include <stdlib.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace cgb {
 
-constexpr int kClipTensors = 448;       // per launch: the table stays under the kernel parameter limit
-constexpr int kClipChunk = 16384;
+// The table of a launch, in the kernel's parameters: a short one for short lists (a launch costs 2.5 us with 40 tensors' worth of
+// parameters and 5 us with 400), a long one up to the parameter limit for the others.
+constexpr int kClipShort = 64, kClipLong = 448;
+constexpr int kClipChunk = 2048;   // elements; what a CTA takes is a run of chunks
 constexpr int kClipThreads = 256;
 
 struct ClipEntry {
@@ -27,8 +32,9 @@ struct ClipEntry {
     long long first_chunk;   // of this launch
     int32_t dtype, out_dtype;
 };
+template <int N>
 struct ClipTable {
-    ClipEntry e[kClipTensors];
+    ClipEntry e[N];
     double* part;            // this launch's CTAs' sums
     const double* all_parts;
     float* norm;
@@ -37,7 +43,8 @@ struct ClipTable {
     float max_norm;
 };
 
-__device__ __forceinline__ int clip_find(const ClipTable& t, long long chunk) {
+template <int N>
+__device__ __forceinline__ int clip_find(const ClipTable<N>& t, long long chunk) {
     int lo = 0, hi = t.count;   // the last tensor whose first chunk is not behind `chunk`; empty tensors have no chunk of their own
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -49,9 +56,17 @@ __device__ __forceinline__ int clip_find(const ClipTable& t, long long chunk) {
 
 // Elements of [p, p + n) before the first 16-byte boundary
 template <typename T>
-__device__ __forceinline__ int clip_head(const T* p, int n) {
-    const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+__device__ __forceinline__ long long clip_head(const T* p, long long n) {
+    const long long h = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
     return h < n ? h : n;
+}
+
+// The chunks of this CTA: an equal share of the list, in one piece
+template <int N>
+__device__ __forceinline__ void clip_share(const ClipTable<N>& t, long long& from, long long& to) {
+    const long long each = t.chunks / gridDim.x, more = t.chunks % gridDim.x, b = blockIdx.x;
+    from = b * each + (b < more ? b : more);
+    to = from + each + (b < more ? 1 : 0);
 }
 
 // A packet's squares: in fp32, and again in fp64 where fp32 leaves its range (|g| above 1.8e19 or all below 1e-15).
@@ -70,22 +85,22 @@ __device__ __forceinline__ double clip_squares(const Vec16<T>& v) {
 }
 
 template <typename T>
-__device__ __forceinline__ double clip_chunk_squares(const T* g, int n) {
-    constexpr int L = Vec16<T>::N, U = 8;
-    const int head = clip_head(g, n), packets = (n - head) / L;
+__device__ __forceinline__ double clip_run_squares(const T* g, long long n) {
+    constexpr int L = Vec16<T>::N, U = 4;
+    const long long head = clip_head(g, n), packets = (n - head) / L;
     double sum = 0.0;
-    for (int i = threadIdx.x; i < head; i += kClipThreads) sum += (double)Elem<T>::to_f32(g[i]) * (double)Elem<T>::to_f32(g[i]);
-    for (int i = head + packets * L + threadIdx.x; i < n; i += kClipThreads) sum += (double)Elem<T>::to_f32(g[i]) * (double)Elem<T>::to_f32(g[i]);
+    for (long long i = threadIdx.x; i < head; i += kClipThreads) sum += (double)Elem<T>::to_f32(g[i]) * (double)Elem<T>::to_f32(g[i]);
+    for (long long i = head + packets * L + threadIdx.x; i < n; i += kClipThreads) sum += (double)Elem<T>::to_f32(g[i]) * (double)Elem<T>::to_f32(g[i]);
     const T* body = g + head;
-    for (int k0 = threadIdx.x; k0 < packets; k0 += kClipThreads * U) {
+    long long k = threadIdx.x;
+    for (; k + (U - 1) * kClipThreads < packets; k += kClipThreads * U) {
         Vec16<T> v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k0 + u * kClipThreads < packets) v[u] = ld_keep(body + (k0 + u * kClipThreads) * L);
+        for (int u = 0; u < U; ++u) v[u] = ld_keep(body + (k + u * kClipThreads) * L);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k0 + u * kClipThreads < packets) sum += clip_squares<T>(v[u]);
+        for (int u = 0; u < U; ++u) sum += clip_squares<T>(v[u]);
     }
+    for (; k < packets; k += kClipThreads) sum += clip_squares<T>(ld_keep(body + k * L));
     return sum;
 }
 
@@ -101,16 +116,19 @@ __device__ __forceinline__ double clip_block_sum(double v, double* scratch) {
     return s;
 }
 
-__global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_constant__ ClipTable t) {
+template <int N>
+__global__ void __launch_bounds__(kClipThreads, 4) clip_norm_kernel(const __grid_constant__ ClipTable<N> t) {
     __shared__ double scratch[kClipThreads / 32];
     double sum = 0.0;
-    for (long long chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
-        const ClipEntry& e = t.e[clip_find(t, chunk)];
-        const long long at = (chunk - e.first_chunk) * kClipChunk;
-        const int n = (int)(e.n - at < kClipChunk ? e.n - at : kClipChunk);
-        if (e.dtype == CG_B200_F32) sum += clip_chunk_squares(static_cast<const float*>(e.in) + at, n);
-        else if (e.dtype == CG_B200_BF16) sum += clip_chunk_squares(static_cast<const __nv_bfloat16*>(e.in) + at, n);
-        else sum += clip_chunk_squares(static_cast<const __half*>(e.in) + at, n);
+    pdl_trigger();
+    long long c, to;
+    for (clip_share(t, c, to); c < to;) {
+        const ClipEntry& e = t.e[clip_find(t, c)];
+        const long long at = (c - e.first_chunk) * kClipChunk, rest = (to - c) * kClipChunk, n = e.n - at < rest ? e.n - at : rest;
+        if (e.dtype == CG_B200_F32) sum += clip_run_squares(static_cast<const float*>(e.in) + at, n);
+        else if (e.dtype == CG_B200_BF16) sum += clip_run_squares(static_cast<const __nv_bfloat16*>(e.in) + at, n);
+        else sum += clip_run_squares(static_cast<const __half*>(e.in) + at, n);
+        c += (n + kClipChunk - 1) / kClipChunk;
     }
     sum = clip_block_sum(sum, scratch);
     if (threadIdx.x == 0) t.part[blockIdx.x] = sum;
@@ -123,70 +141,107 @@ __device__ __forceinline__ double clip_norm(const double* parts, int n, double* 
     return sqrt(clip_block_sum(s, scratch));
 }
 
+// A thread's piece is one 16-byte packet of the wider side, so that a warp's stores are contiguous: 16-bit gradients that become fp32 are
+// read 8 bytes at a time.
 template <typename T, typename O>
-__device__ __forceinline__ void clip_chunk_scale(const T* g, O* o, int n, float factor) {
-    constexpr int L = Vec16<T>::N, M = Vec16<O>::N, R = L / M, U = 8;
-    const int head = clip_head(g, n);
-    const bool vec = ((reinterpret_cast<uintptr_t>(o + head)) & 15) == 0;   // both sides reach a boundary at the same element
-    const int packets = vec ? (n - head) / L : 0, loose = vec ? head : 0;
-    for (int i = threadIdx.x; i < loose; i += kClipThreads) o[i] = Elem<O>::from_f32(Elem<T>::to_f32(g[i]) * factor);
-    for (int i = loose + packets * L + threadIdx.x; i < n; i += kClipThreads) o[i] = Elem<O>::from_f32(Elem<T>::to_f32(g[i]) * factor);
+__device__ __forceinline__ void clip_run_scale(const T* g, O* o, long long n, float factor) {
+    constexpr int E = Vec16<O>::N, U = 4;   // elements of a piece; sizeof(O) >= sizeof(T)
+    typedef typename std::conditional<E * sizeof(T) == 16, int4, int2>::type Raw;
+    const long long head = clip_head(o, n);
+    const bool vec = (reinterpret_cast<uintptr_t>(g + head) & (sizeof(Raw) - 1)) == 0;   // both sides reach a boundary at the same element
+    const long long pieces = vec ? (n - head) / E : 0, loose = vec ? head : 0;
+    for (long long i = threadIdx.x; i < loose; i += kClipThreads) o[i] = Elem<O>::from_f32(Elem<T>::to_f32(g[i]) * factor);
+    for (long long i = loose + pieces * E + threadIdx.x; i < n; i += kClipThreads) o[i] = Elem<O>::from_f32(Elem<T>::to_f32(g[i]) * factor);
     const T* gb = g + head;
     O* ob = o + head;
-    for (int k0 = threadIdx.x; k0 < packets; k0 += kClipThreads * U) {
-        Vec16<T> v[U];
+    auto put = [&](long long k, const Raw& raw) {
+        Vec16<T> v;
+        *reinterpret_cast<Raw*>(&v) = raw;
+        float f[Vec16<T>::N], q[E];
+        unpack16<T>(v, f);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k0 + u * kClipThreads < packets) v[u] = ld_stream(gb + (k0 + u * kClipThreads) * L);
+        for (int i = 0; i < E; ++i) q[i] = f[i] * factor;
+        st_stream(ob + k * E, pack16<O>(q));
+    };
+    long long k = pieces - 1 - threadIdx.x;
+    for (; k >= (U - 1) * kClipThreads; k -= kClipThreads * U) {
+        Raw raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (k0 + u * kClipThreads < packets) {
-                float f[L];
-                unpack16<T>(v[u], f);
+        for (int u = 0; u < U; ++u) raw[u] = __ldcs(reinterpret_cast<const Raw*>(gb + (k - u * kClipThreads) * E));
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float q[M];
-#pragma unroll
-                    for (int i = 0; i < M; ++i) q[i] = f[r * M + i] * factor;
-                    st_stream(ob + (k0 + u * kClipThreads) * L + r * M, pack16<O>(q));
-                }
-            }
+        for (int u = 0; u < U; ++u) put(k - u * kClipThreads, raw[u]);
     }
+    for (; k >= 0; k -= kClipThreads) put(k, __ldcs(reinterpret_cast<const Raw*>(gb + k * E)));
 }
 
-__global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_constant__ ClipTable t) {
+template <int N>
+__global__ void __launch_bounds__(kClipThreads, 4) clip_scale_kernel(const __grid_constant__ ClipTable<N> t) {
     __shared__ double scratch[kClipThreads / 32];
+    pdl_trigger();
+    pdl_wait();
     const double norm = clip_norm(t.all_parts, t.n_parts, scratch);
     if (t.norm && blockIdx.x == 0 && threadIdx.x == 0) *t.norm = (float)norm;
     const double ratio = (double)t.max_norm / (norm + 1e-6);
     const float factor = ratio >= 1.0 ? 1.0f : (float)ratio;   // a norm that is not a number gives such a factor
-    for (long long c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const long long chunk = t.chunks - 1 - c;
-        const ClipEntry& e = t.e[clip_find(t, chunk)];
+    long long from, to;
+    for (clip_share(t, from, to); to > from;) {
+        const ClipEntry& e = t.e[clip_find(t, to - 1)];
+        const long long c = e.first_chunk > from ? e.first_chunk : from, at = (c - e.first_chunk) * kClipChunk, rest = (to - c) * kClipChunk;
+        const long long n = e.n - at < rest ? e.n - at : rest;
+        to = c;
         if (e.in == e.out && factor == 1.0f) continue;   // already there
-        const long long at = (chunk - e.first_chunk) * kClipChunk;
-        const int n = (int)(e.n - at < kClipChunk ? e.n - at : kClipChunk);
         if (e.dtype == CG_B200_F32) {
-            clip_chunk_scale(static_cast<const float*>(e.in) + at, static_cast<float*>(e.out) + at, n, factor);
+            clip_run_scale(static_cast<const float*>(e.in) + at, static_cast<float*>(e.out) + at, n, factor);
         } else if (e.dtype == CG_B200_BF16) {
             const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(e.in) + at;
-            if (e.out_dtype == CG_B200_F32) clip_chunk_scale(g, static_cast<float*>(e.out) + at, n, factor);
-            else clip_chunk_scale(g, static_cast<__nv_bfloat16*>(e.out) + at, n, factor);
+            if (e.out_dtype == CG_B200_F32) clip_run_scale(g, static_cast<float*>(e.out) + at, n, factor);
+            else clip_run_scale(g, static_cast<__nv_bfloat16*>(e.out) + at, n, factor);
         } else {
             const __half* g = static_cast<const __half*>(e.in) + at;
-            if (e.out_dtype == CG_B200_F32) clip_chunk_scale(g, static_cast<float*>(e.out) + at, n, factor);
-            else clip_chunk_scale(g, static_cast<__half*>(e.out) + at, n, factor);
+            if (e.out_dtype == CG_B200_F32) clip_run_scale(g, static_cast<float*>(e.out) + at, n, factor);
+            else clip_run_scale(g, static_cast<__half*>(e.out) + at, n, factor);
         }
     }
 }
 
 __global__ void __launch_bounds__(kClipThreads) clip_norm_only_kernel(const double* parts, int n, float* norm) {
     __shared__ double scratch[kClipThreads / 32];
+    pdl_trigger();
+    pdl_wait();
     const double v = clip_norm(parts, n, scratch);
     if (threadIdx.x == 0) *norm = (float)v;
 }
 
 static long long clip_grid_cap() { return (long long)sm_count() * 4; }
+
+// Nothing may be written twice, and nothing written may be another's input: a tensor is scaled in place, or into memory of its own. The
+// address ranges are sorted and swept once.
+struct ClipRange {
+    uintptr_t from, to;
+    bool written;
+};
+static int clip_check_overlap(const cg_b200_grad* g, int64_t count) {
+    ClipRange few[2 * kClipShort];
+    ClipRange* r = few;
+    if (count > kClipShort && !(r = static_cast<ClipRange*>(malloc((size_t)count * 2 * sizeof(ClipRange))))) return CG_B200_ERR_INVALID_ARG;
+    int64_t n = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (g[i].n == 0) continue;
+        const uintptr_t in = reinterpret_cast<uintptr_t>(g[i].in), out = reinterpret_cast<uintptr_t>(g[i].out);
+        r[n++] = {out, out + (size_t)g[i].n * dtype_bytes(g[i].out_dtype), true};
+        if (in != out || g[i].dtype != g[i].out_dtype) r[n++] = {in, in + (size_t)g[i].n * dtype_bytes(g[i].dtype), false};
+    }
+    std::sort(r, r + n, [](const ClipRange& a, const ClipRange& b) { return a.from < b.from; });
+    uintptr_t read_to = 0, written_to = 0;
+    bool bad = false;
+    for (int64_t i = 0; i < n && !bad; ++i) {
+        bad = r[i].from < written_to || (r[i].written && r[i].from < read_to);
+        uintptr_t& to = r[i].written ? written_to : read_to;
+        if (r[i].to > to) to = r[i].to;
+    }
+    if (r != few) free(r);
+    return bad ? CG_B200_ERR_INVALID_ARG : CG_B200_OK;
+}
 
 static int clip_check(const cg_b200_grad* g, int64_t count, bool scale) {
     if (count < 0 || count > (1 << 20)) return CG_B200_ERR_INVALID_ARG;
@@ -199,61 +254,64 @@ static int clip_check(const cg_b200_grad* g, int64_t count, bool scale) {
         if (!aligned_to(g[i].in, dtype_bytes(g[i].dtype))) return CG_B200_ERR_MISALIGNED;
         if (!scale) continue;
         if (!aligned_to(g[i].out, dtype_bytes(g[i].out_dtype))) return CG_B200_ERR_MISALIGNED;
-        // in place, or apart: a shifted or widened copy over its own input would read what it has overwritten
-        const uintptr_t a = reinterpret_cast<uintptr_t>(g[i].in), b = reinterpret_cast<uintptr_t>(g[i].out);
-        const uintptr_t ae = a + (size_t)g[i].n * dtype_bytes(g[i].dtype), be = b + (size_t)g[i].n * dtype_bytes(g[i].out_dtype);
-        if (a < be && b < ae && !(a == b && g[i].dtype == g[i].out_dtype)) return CG_B200_ERR_INVALID_ARG;
     }
-    return CG_B200_OK;
+    return scale ? clip_check_overlap(g, count) : CG_B200_OK;
 }
 
 static size_t clip_workspace(int64_t count) {
-    const int64_t launches = (count + kClipTensors - 1) / kClipTensors;
+    const int64_t launches = (count + kClipLong - 1) / kClipLong;
     return (size_t)(launches > 0 ? launches : 1) * (size_t)clip_grid_cap() * sizeof(double);
 }
 
-// The launches over the list, kClipTensors at a time: sums (scale false) or the scaled copies.
-static int clip_run(const cg_b200_grad* g, int64_t count, float max_norm, float* norm, double* ws, bool scale, cudaStream_t s) {
-    long long n_parts = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        long long at = 0;
-        for (int64_t i0 = 0; i0 < count; i0 += kClipTensors) {
-            ClipTable t;
-            t.count = 0;
-            t.chunks = 0;
-            for (int64_t i = i0; i < count && i < i0 + kClipTensors; ++i) {
-                if (g[i].n == 0) continue;
-                ClipEntry& e = t.e[t.count++];
-                e.in = g[i].in;
-                e.out = g[i].out;
-                e.n = g[i].n;
-                e.dtype = g[i].dtype;
-                e.out_dtype = g[i].out_dtype;
-                e.first_chunk = t.chunks;
-                t.chunks += (g[i].n + kClipChunk - 1) / kClipChunk;
-            }
-            if (t.count == 0) continue;
-            const long long cap = clip_grid_cap();
-            const unsigned grid = (unsigned)(t.chunks < cap ? t.chunks : cap);
-            t.part = ws + at;
-            t.all_parts = ws;
-            t.n_parts = (int)n_parts;
-            t.norm = at == 0 ? norm : nullptr;
-            t.max_norm = max_norm;
-            if (pass == 0) clip_norm_kernel<<<grid, kClipThreads, 0, s>>>(t);
-            else clip_scale_kernel<<<grid, kClipThreads, 0, s>>>(t);
+// The launches over the list, N tensors at a time: sums, or the scaled copies. *parts: sums written so far, or all of them.
+template <int N>
+static int clip_pass(const cg_b200_grad* g, int64_t count, float max_norm, float* norm, double* ws, bool scale, int* parts, cudaStream_t s) {
+    ClipTable<N> t;
+    int at = 0;
+    for (int64_t i0 = 0; i0 < count; i0 += N) {
+        t.count = 0;
+        t.chunks = 0;
+        for (int64_t i = i0; i < count && i < i0 + N; ++i) {
+            if (g[i].n == 0) continue;
+            ClipEntry& e = t.e[t.count++];
+            e.in = g[i].in;
+            e.out = g[i].out;
+            e.n = g[i].n;
+            e.dtype = g[i].dtype;
+            e.out_dtype = g[i].out_dtype;
+            e.first_chunk = t.chunks;
+            t.chunks += (g[i].n + kClipChunk - 1) / kClipChunk;
+        }
+        if (t.count == 0) continue;
+        const long long cap = clip_grid_cap();
+        const unsigned grid = (unsigned)(t.chunks < cap ? t.chunks : cap);
+        t.part = ws + at;
+        t.all_parts = ws;
+        t.n_parts = *parts;
+        t.norm = at == 0 ? norm : nullptr;
+        t.max_norm = max_norm;
+        if (!scale) {
+            clip_norm_kernel<N><<<grid, kClipThreads, 0, s>>>(t);
             CGB_CUDA(cudaGetLastError());
-            at += grid;
+        } else {
+            CGB_CUDA(launch_pdl(clip_scale_kernel<N>, grid, kClipThreads, 0, s, t));
         }
-        if (pass == 0) {
-            n_parts = at;
-            if (!scale || n_parts == 0) {
-                clip_norm_only_kernel<<<1, kClipThreads, 0, s>>>(ws, (int)n_parts, norm);
-                CGB_CUDA(cudaGetLastError());
-                return CG_B200_OK;
-            }
-        }
+        at += (int)grid;
     }
+    if (!scale) *parts = at;
+    return CG_B200_OK;
+}
+
+static int clip_run(const cg_b200_grad* g, int64_t count, float max_norm, float* norm, double* ws, bool scale, cudaStream_t s) {
+    auto pass = [&](bool second, int* parts) {
+        return count <= kClipShort ? clip_pass<kClipShort>(g, count, max_norm, norm, ws, second, parts, s)
+                                   : clip_pass<kClipLong>(g, count, max_norm, norm, ws, second, parts, s);
+    };
+    int parts = 0;
+    const int st = pass(false, &parts);
+    if (st) return st;
+    if (scale && parts > 0) return pass(true, &parts);
+    CGB_CUDA(launch_pdl(clip_norm_only_kernel, 1, kClipThreads, 0, s, (const double*)ws, parts, norm));
     return CG_B200_OK;
 }
 

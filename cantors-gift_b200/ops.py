@@ -3,7 +3,9 @@
 PyTorch is used for device memory and streams only; every computation is a cg_b200_* call.
 bf16 host arrays travel as uint16 bit patterns.
 """
+import array
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -132,6 +134,14 @@ def _raw_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(op, index, *sizes):
+    """cg_b200_<op>_workspace_bytes(*sizes) on device `index`, the current one."""
+    need = C.c_size_t(0)
+    check(getattr(lib(), f"cg_b200_{op}_workspace_bytes")(*sizes, C.byref(need)), f"{op}_workspace_bytes")
+    return need.value
+
+
 def _dtype_code(dtype):
     code = DTYPE_OF_TORCH.get(dtype)
     if code is None:
@@ -181,7 +191,7 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, r
     else:
         _check_like(out, shape, x.dtype, "out")
     if mean is None:
-        mean = torch.empty(lead, dtype=torch.float32, device=x.device)
+        mean = x.new_empty(lead, dtype=torch.float32)
     else:
         _check_like(mean, lead, torch.float32, "mean")
     if rstd is None:
@@ -215,10 +225,8 @@ def layernorm_backward(dy, x, mean, rstd, gamma=None, bias=True, dx=None, dgamma
         dbeta = torch.empty_like(gamma) if dbeta is None and bias else dbeta
     ws, ws_bytes = None, 0
     if dgamma is not None or dbeta is not None:
-        need = C.c_size_t(0)
-        check(lib().cg_b200_layernorm_backward_workspace_bytes(rows, cols, C.byref(need)), "layernorm_backward_workspace_bytes")
-        ws_bytes = need.value
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        ws_bytes = _workspace_bytes("layernorm_backward", x.get_device(), rows, cols)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
     check(lib().cg_b200_layernorm_backward(dt, pt, dy.data_ptr(), x.data_ptr(), _addr(gamma), mean.data_ptr(), rstd.data_ptr(),
                                            dx.data_ptr(), _addr(dgamma), _addr(dbeta), rows, cols, _addr(ws), ws_bytes,
                                            _raw_stream(x.get_device())), "layernorm_backward")
@@ -251,7 +259,7 @@ def embedding(table, ids, scale=1.0, dtype=None, out=None, stream=None):
     vocab, cols = table.shape
     shape = (*ids.shape, cols)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=table.device)
+        out = table.new_empty(shape, dtype=dtype)
     else:
         _check_like(out, shape, dtype, "out")
     check(lib().cg_b200_embedding(dt, tt, table.data_ptr(), vocab, cols, ids.data_ptr(), idb, ids.numel(), scale, out.data_ptr(),
@@ -277,31 +285,47 @@ def embedding_backward(dy, ids, vocab, scale=1.0, padding_id=None, dtype=None, o
     dt, gt, idb = _dtype_code(dy.dtype), _dtype_code(dtype), _id_bytes(ids)
     n, cols = ids.numel(), dy.shape[-1]
     if out is None:
-        out = torch.empty((vocab, cols), dtype=dtype, device=dy.device)
+        out = dy.new_empty((vocab, cols), dtype=dtype)
     else:
         _check_like(out, (vocab, cols), dtype, "out")
-    need = C.c_size_t(0)
-    check(lib().cg_b200_embedding_backward_workspace_bytes(n, vocab, cols, C.byref(need)), "embedding_backward_workspace_bytes")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
+    index = dy.get_device()
+    need = _workspace_bytes("embedding_backward", index, n, vocab, cols)
+    ws = dy.new_empty(need, dtype=torch.uint8)
     check(lib().cg_b200_embedding_backward(dt, gt, dy.data_ptr(), ids.data_ptr(), idb, n, scale,
                                            -1 if padding_id is None else padding_id, int(accumulate), out.data_ptr(), vocab, cols,
-                                           ws.data_ptr(), need.value, _raw_stream(dy.get_device())), "embedding_backward")
+                                           ws.data_ptr(), need, _raw_stream(index)), "embedding_backward")
     return out
 
 
+_contiguous, _device_index, _address, _numel = (torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.data_ptr,
+                                                torch.Tensor.numel)
+
+
+def _grad_words(tensors, index):
+    """(addresses, sizes, type codes) of a list of contiguous tensors on CUDA device `index`."""
+    if index < 0 or set(map(_device_index, tensors)) != {index} or not all(map(_contiguous, tensors)):
+        raise ValueError("cg_b200 ops take contiguous CUDA tensors on one device")
+    codes = [DTYPE_OF_TORCH.get(t.dtype) for t in tensors]
+    if None in codes:
+        raise ValueError("gradients are float32, bfloat16 or float16")
+    return list(map(_address, tensors)), list(map(_numel, tensors)), codes
+
+
 def _grad_table(grads, outs):
-    """The C ABI's table of a list of tensors, four 64-bit words each (cg_b200_grad). Empty tensors may be among them."""
-    index, words = grads[0].get_device(), []
-    for g, o in zip(grads, outs):
-        if index < 0 or g.get_device() != index or not g.is_contiguous():
-            raise ValueError("cg_b200 ops take contiguous CUDA tensors on one device")
-        if o is not g:
-            if o.get_device() != index or not o.is_contiguous():
-                raise ValueError("cg_b200 ops take contiguous CUDA tensors on one device")
-            if o.shape != g.shape:
-                raise ValueError(f"output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
-        words += (g.data_ptr(), o.data_ptr(), g.numel(), _dtype_code(g.dtype) | _dtype_code(o.dtype) << 32)
-    return (C.c_int64 * len(words))(*words), words
+    """The C ABI's table of a list of tensors, four 64-bit words each (cg_b200_grad)."""
+    index = grads[0].get_device()
+    at, sizes, codes = _grad_words(grads, index)
+    to, out_codes = at, codes
+    if outs is not None:
+        if len(outs) != len(grads):
+            raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
+        to, out_sizes, out_codes = _grad_words(outs, index)
+        if out_sizes != sizes:
+            raise ValueError("each output must have as many elements as its gradient")
+    words = [0] * (4 * len(grads))
+    words[0::4], words[1::4], words[2::4] = at, to, sizes
+    words[3::4] = [a | b << 32 for a, b in zip(codes, out_codes)]
+    return array.array("q", words)
 
 
 def grad_norm(grads, norm=None, stream=None):
@@ -311,7 +335,8 @@ def grad_norm(grads, norm=None, stream=None):
 
 def clip_grad_norm(grads, max_norm, out=None, norm=None, stream=None):
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)) and returns their norm before it (0-dim fp32, on the device;
-    nothing waits for the GPU). In place, or into `out`: tensors of the same shapes, each of its gradient's dtype or fp32."""
+    nothing waits for the GPU). In place, or into `out`: one tensor for each, of as many elements, of its gradient's dtype or
+    fp32, in memory of its own. No tensor may be in the list twice."""
     return _norm_call(list(grads), max_norm, out, norm, stream)
 
 
@@ -323,31 +348,19 @@ def _norm_call(grads, max_norm, out, norm, stream):
     if ctx is not None:
         with ctx:
             return _norm_call(grads, max_norm, out, norm, None)
-    outs = grads if out is None else list(out)
-    if len(outs) != len(grads):
-        raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
-    table, words = _grad_table(grads, outs)
-    if max_norm is not None:
-        # no tensor may be written twice, and no output may be another gradient
-        pairs = [(i, o) for i, o, n in zip(words[::4], words[1::4], words[2::4]) if n]
-        written = {o for _, o in pairs}
-        if len(written) < len(pairs):
-            raise ValueError("a tensor is in the list twice")
-        if out is not None and any(i != o and i in written for i, o in pairs):
-            raise ValueError("an output is another gradient of the list")
+    table = _grad_table(grads, None if out is None else list(out))
     if norm is None:
-        norm = torch.empty((), dtype=torch.float32, device=first.device)
+        norm = first.new_empty((), dtype=torch.float32)
     else:
         _require_one_device(first, norm)
         _check_like(norm, (), torch.float32, "norm")
-    need = C.c_size_t(0)
-    check(lib().cg_b200_grad_norm_workspace_bytes(len(grads), C.byref(need)), "grad_norm_workspace_bytes")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=first.device)
-    grad_p, at = C.cast(table, C.POINTER(capi.Grad)), _raw_stream(first.get_device())
+    index, words = first.get_device(), table.buffer_info()[0]
+    need = _workspace_bytes("grad_norm", index, len(grads))
+    ws = first.new_empty(need, dtype=torch.uint8)
     if max_norm is None:
-        check(lib().cg_b200_grad_norm(grad_p, len(grads), norm.data_ptr(), ws.data_ptr(), need.value, at), "grad_norm")
+        check(lib().cg_b200_grad_norm(words, len(grads), norm.data_ptr(), ws.data_ptr(), need, _raw_stream(index)), "grad_norm")
     else:
-        check(lib().cg_b200_clip_grad_norm(grad_p, len(grads), max_norm, norm.data_ptr(), ws.data_ptr(), need.value, at),
+        check(lib().cg_b200_clip_grad_norm(words, len(grads), max_norm, norm.data_ptr(), ws.data_ptr(), need, _raw_stream(index)),
               "clip_grad_norm")
     return norm
 

@@ -455,17 +455,21 @@ def test_clip_no_write_outside(ops):
 
 def test_clip_refusals(ops):
     g = normal(64)
-    for bad in (lambda: ops.clip_grad_norm([], 1.0), lambda: ops.clip_grad_norm([g, g], 1.0),
-                lambda: ops.clip_grad_norm([g], 1.0, out=[]), lambda: ops.clip_grad_norm([g], 1.0, out=[normal(63)]),
-                lambda: ops.clip_grad_norm([g.view(8, 8).t()], 1.0), lambda: ops.clip_grad_norm([g.double()], 1.0),
-                lambda: ops.clip_grad_norm([g, normal(64, seed=1)], 1.0, out=[torch.empty_like(g), g])):
+    for bad in (lambda: ops.clip_grad_norm([], 1.0), lambda: ops.clip_grad_norm([g], 1.0, out=[]),
+                lambda: ops.clip_grad_norm([g], 1.0, out=[normal(63)]), lambda: ops.clip_grad_norm([g.view(8, 8).t()], 1.0),
+                lambda: ops.clip_grad_norm([g.double()], 1.0), lambda: ops.clip_grad_norm([g, g.cpu()], 1.0)):
         with pytest.raises(ValueError):
             bad()
     from cantors_gift_b200 import CgB200Error
-    with pytest.raises(CgB200Error):
-        ops.clip_grad_norm([g], -1.0)
-    with pytest.raises(CgB200Error):
-        ops.clip_grad_norm([g], 1.0, out=[torch.empty(64, dtype=torch.float16, device="cuda")])
+    other, half = normal(64, seed=1), torch.empty(64, dtype=torch.float16, device="cuda")
+    for bad in (lambda: ops.clip_grad_norm([g], -1.0), lambda: ops.clip_grad_norm([g], 1.0, out=[half]),
+                lambda: ops.clip_grad_norm([g, g], 1.0),                                          # scaled twice
+                lambda: ops.clip_grad_norm([g, g[8:16]], 1.0),                                     # in part
+                lambda: ops.clip_grad_norm([g, other], 1.0, out=[torch.empty_like(g), g]),         # over another gradient
+                lambda: ops.clip_grad_norm([g, other], 1.0, out=[half.float()] * 2)):
+        with pytest.raises(CgB200Error):
+            bad()
+    assert float(ops.grad_norm([g, g])) > 0   # reading one twice is no harm
 
 
 # ---- streams, graphs, and the operators one after another ----------------------------------------------------

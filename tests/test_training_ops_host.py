@@ -120,6 +120,10 @@ def test_clip_refusals(cgb):
     assert clip(table(out_dtype=capi.F16)) == capi.ERR_INVALID_ARG
     assert clip(table(out_dtype=capi.F32)) == capi.ERR_INVALID_ARG               # widened over its own input
     assert clip(table(out=(1 << 16) + 2)) == capi.ERR_INVALID_ARG                # shifted over its own input
+    assert clip(table(in_=1 << 18, out=1 << 18)) == capi.ERR_INVALID_ARG         # the same tensor twice
+    assert clip(table(out=(1 << 18) + 100)) == capi.ERR_INVALID_ARG              # into the other gradient
+    assert clip(table(out=(1 << 18) + 198)) == capi.ERR_INVALID_ARG              # by its last element
+    assert clip(table(out=(1 << 18) + 200), ws=None) == capi.ERR_WORKSPACE       # beside it is fine
     assert clip(table(), ws=None) == capi.ERR_WORKSPACE
     assert clip(table(), ws_bytes=need.value - 1) == capi.ERR_WORKSPACE
     t = table(out_dtype=77, out=None)
