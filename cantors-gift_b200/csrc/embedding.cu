@@ -10,7 +10,10 @@
 // timing - and walks the sorted list in chunks of 32 pairs. A warp takes a chunk for 512 bytes of columns: it adds the rows of every id
 // that begins in the chunk, in fp32 registers, following the last one into the next chunk, and writes the id's table row. Only an id
 // whose pairs cover a whole chunk and reach beyond it is added by several warps: their sums go to the workspace and a last kernel joins
-// them in order. The table rows that no id names are zeroed beside the sums.
+// them in order. The table rows that no id names are cleared beside the sort, as far as that takes no longer than the sort, and beside
+// the sums.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace cgb {
@@ -117,7 +120,19 @@ struct SortParams {
     uint32_t* joins;        // length of the list of joins, cleared
     long long n, vocab, padding;
     int tiles, bins, shift, shift_next;
+    char* zero_from;        // what the CTAs that do not sort clear meanwhile
+    long long zero_bytes;
 };
+
+// Clears [from, from + bytes): thread `at` of `of`.
+__device__ __forceinline__ void zero_range(char* from, long long bytes, long long at, long long of) {
+    const long long to_edge = (16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15, head = to_edge < bytes ? to_edge : bytes;
+    const long long packets = (bytes - head) / 16;
+    if (at < head) from[at] = 0;
+    for (long long i = head + packets * 16 + at; i < bytes; i += of) from[i] = 0;
+    int4* body = reinterpret_cast<int4*>(from + head);
+    for (long long i = at; i < packets; i += of) __stcs(body + i, make_int4(0, 0, 0, 0));
+}
 
 template <typename I>
 __device__ __forceinline__ uint32_t sort_key(const SortParams& p, long long i) {
@@ -154,17 +169,25 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {
     return v;
 }
 
-// A warp's pairs of one round of 32: their ranks among the equal digits of this warp so far, counted in `cnt` (one counter per bin).
-template <typename C>
-__device__ __forceinline__ uint32_t sort_rank(C* cnt, uint32_t digit, bool live, int lane) {
-    const unsigned peers = __match_any_sync(0xffffffffu, live ? digit : 0xffffffffu);
-    const int below = __popc(peers & ((1u << lane) - 1u));
-    uint32_t before = 0;
-    if (live) before = cnt[digit];
-    __syncwarp();
-    if (live && below == 0) cnt[digit] = (C)(before + __popc(peers));
-    __syncwarp();
-    return before + below;
+// Ranks of a warp's pairs, ROUNDS times 32 in order, among the equal digits of this warp, counted in `cnt` (one counter per bin).
+// Rounds that are not there (live false in every lane) count nothing.
+template <int ROUNDS, typename C>
+__device__ __forceinline__ void sort_rank(C* cnt, const uint32_t (&key)[ROUNDS], const bool (&live)[ROUNDS], int shift, int bins, int lane,
+                                          uint32_t (&rank)[ROUNDS]) {
+    unsigned peers[ROUNDS];   // lanes with the same digit: these do not wait for one another, the counters below do
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) peers[r] = __match_any_sync(0xffffffffu, live[r] ? (key[r] >> shift) & (bins - 1) : 0xffffffffu);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const uint32_t digit = (key[r] >> shift) & (bins - 1);
+        const int below = __popc(peers[r] & ((1u << lane) - 1u));
+        uint32_t before = 0;
+        if (live[r]) before = cnt[digit];
+        __syncwarp();
+        if (live[r] && below == 0) cnt[digit] = (C)(before + __popc(peers[r]));
+        __syncwarp();
+        rank[r] = before + below;
+    }
 }
 
 // One pass: ranks within the tile, the tile's place in every bin from the counts of all tiles, the scatter, and the next pass's counts.
@@ -200,9 +223,10 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_scatter_kernel(const __g
             if (t < blockIdx.x) earlier += c;
         }
     }
+    bool live[kSortRounds];
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)
-        rank[r] = sort_rank(cnt[warp], (key[r] >> p.shift) & (p.bins - 1), first + r * 32 + lane < p.n, lane);
+    for (int r = 0; r < kSortRounds; ++r) live[r] = first + r * 32 + lane < p.n;
+    sort_rank<kSortRounds>(cnt[warp], key, live, p.shift, p.bins, lane, rank);
     const uint32_t scan = warp_scan(total, lane);
     if (lane == 31) warp_total[warp] = scan;
     __syncthreads();
@@ -222,97 +246,136 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_scatter_kernel(const __g
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
-        const bool live = first + r * 32 + lane < p.n;
         const uint32_t digit = (key[r] >> p.shift) & (p.bins - 1);
         uint32_t to = 0;
-        if (live) {
+        if (live[r]) {
             to = base[digit] + cnt[warp][digit] + rank[r];
             p.key_out[to] = key[r];
             p.pos_out[to] = pos[r];
         }
         if (p.count_next) {
             // frequent ids share a counter: one addition per warp and counter
-            const uint32_t at = live ? (to / kSortTile) * p.bins + ((key[r] >> p.shift_next) & (p.bins - 1)) : 0xffffffffu;
+            const uint32_t at = live[r] ? (to / kSortTile) * p.bins + ((key[r] >> p.shift_next) & (p.bins - 1)) : 0xffffffffu;
             const unsigned peers = __match_any_sync(0xffffffffu, at);
-            if (live && lane == __ffs(peers) - 1) atomicAdd(&p.count_next[at], (uint32_t)__popc(peers));
+            if (live[r] && lane == __ffs(peers) - 1) atomicAdd(&p.count_next[at], (uint32_t)__popc(peers));
         }
     }
 }
 
-// Up to kSortSmall pairs in one CTA: every pass through shared memory, one launch instead of one per pass and one for the counts.
-constexpr int kSortSmall = 8192, kSmallWarps = 32, kSmallRounds = kSortSmall / (32 * kSmallWarps);
-struct SortSmall {
-    uint32_t key[kSortSmall];
-    uint16_t pos[kSortSmall];
-    uint16_t cnt[kSmallWarps][kSortBins];
-    uint32_t base[kSortBins];
-    uint32_t warp_total[kSmallWarps];
+// Up to 16 * 8192 pairs by one cluster of CTAs, in one launch: a pass's pairs go from registers through the shared memory of the CTA
+// that owns their place, and the counts of all CTAs are read there too, so nothing but the ids and the result is in global memory.
+// CTA c owns the places c * span .. (c + 1) * span - 1, span = 1024 * ROUNDS; a thread holds ROUNDS pairs.
+// The sort keeps sixteen SMs busy and memory idle, so the other clusters of the launch clear the end of the table's gradient meanwhile.
+constexpr int kClusterWarps = 32, kClusterThreads = kClusterWarps * 32;
+template <int ROUNDS> struct SortShared {
+    uint2 pair[ROUNDS * kClusterThreads];
+    uint16_t cnt[kClusterWarps][kSortBins];
+    uint32_t hist[kSortBins], base[kSortBins], warp_total[kClusterWarps];
 };
-template <typename I>
-__global__ void __launch_bounds__(kSmallWarps * 32) sort_small_kernel(const __grid_constant__ SortParams p, int passes, int digit_bits) {
+template <typename I, int ROUNDS>
+__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __grid_constant__ SortParams p, int passes, int digit_bits) {
     extern __shared__ float4 sort_smem4[];
-    SortSmall& sm = *reinterpret_cast<SortSmall*>(sort_smem4);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (int)p.n;
-    // the warps share the pairs evenly, in whole rounds
-    const int rounds = (n + 32 * kSmallWarps - 1) / (32 * kSmallWarps), first = warp * rounds * 32 + lane;
+    typedef SortShared<ROUNDS> Shared;
+    Shared& sm = *reinterpret_cast<Shared*>(sort_smem4);
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), n = (int)p.n;
+    constexpr int span = ROUNDS * kClusterThreads;
+    const int local = warp * (32 * ROUNDS) + lane, first = me * span + local;
+    const uint32_t low = p.bins - 1;
+    uint32_t key[ROUNDS], pos[ROUNDS], rank[ROUNDS];
+    bool live[ROUNDS];
     pdl_trigger();
-    uint32_t key[kSmallRounds], rank[kSmallRounds];
-    uint32_t pos[kSmallRounds];
-    pdl_wait();
+    if (blockIdx.x >= ctas)
+        return zero_range(p.zero_from, p.zero_bytes, (long long)(blockIdx.x - ctas) * kClusterThreads + threadIdx.x,
+                          (long long)(gridDim.x - ctas) * kClusterThreads);
 #pragma unroll
-    for (int r = 0; r < kSmallRounds; ++r) {
-        const int i = first + r * 32;
-        pos[r] = (uint32_t)i;
-        key[r] = r < rounds && i < n ? sort_key<I>(p, i) : 0xffffffffu;
+    for (int r = 0; r < ROUNDS; ++r) {
+        live[r] = first + r * 32 < n;
+        pos[r] = (uint32_t)(first + r * 32);
+        key[r] = live[r] ? sort_key<I>(p, first + r * 32) : 0u;
     }
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * digit_bits;
-        for (int b = threadIdx.x; b < p.bins * kSmallWarps; b += blockDim.x) sm.cnt[b / p.bins][b % p.bins] = 0;
+        for (int b = threadIdx.x; b < kSortBins * kClusterWarps / 8; b += kClusterThreads) reinterpret_cast<uint4*>(sm.cnt)[b] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r)
-            if (r < rounds) rank[r] = sort_rank(sm.cnt[warp], (key[r] >> shift) & (p.bins - 1), first + r * 32 < n, lane);
+        sort_rank<ROUNDS>(sm.cnt[warp], key, live, shift, p.bins, lane, rank);
         __syncthreads();
-        uint32_t total = 0;
         if (threadIdx.x < p.bins) {
+            uint32_t run = 0;
 #pragma unroll
-            for (int w = 0; w < kSmallWarps; ++w) {
+            for (int w = 0; w < kClusterWarps; ++w) {
                 const uint32_t c = sm.cnt[w][threadIdx.x];
-                sm.cnt[w][threadIdx.x] = (uint16_t)total;
-                total += c;
+                sm.cnt[w][threadIdx.x] = (uint16_t)run;
+                run += c;
             }
+            sm.hist[threadIdx.x] = run;
         }
+        cluster.sync();   // every CTA's counts are there, and its pairs of the last pass have been taken out
+        uint32_t total = 0, earlier = 0;
+        if (threadIdx.x < p.bins)
+#pragma unroll 16
+            for (int c = 0; c < ctas; ++c) {
+                const uint32_t v = *cluster.map_shared_rank(&sm.hist[threadIdx.x], c);
+                total += v;
+                if (c < me) earlier += v;
+            }
         const uint32_t scan = warp_scan(total, lane);
         if (lane == 31) sm.warp_total[warp] = scan;
         __syncthreads();
         if (threadIdx.x < p.bins) {
             uint32_t lower = 0;
             for (int w = 0; w < warp; ++w) lower += sm.warp_total[w];
-            sm.base[threadIdx.x] = lower + scan - total;
+            sm.base[threadIdx.x] = lower + scan - total + earlier;
         }
         __syncthreads();
+        const bool last = pass + 1 == passes;
 #pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r)
-            if (r < rounds && first + r * 32 < n) {
-                const uint32_t digit = (key[r] >> shift) & (p.bins - 1), to = sm.base[digit] + sm.cnt[warp][digit] + rank[r];
-                sm.key[to] = key[r];
-                sm.pos[to] = (uint16_t)pos[r];
+        for (int r = 0; r < ROUNDS; ++r)
+            if (live[r]) {
+                const uint32_t digit = (key[r] >> shift) & low, to = sm.base[digit] + sm.cnt[warp][digit] + rank[r];
+                if (last) {
+                    p.key_out[to] = key[r];
+                    p.pos_out[to] = pos[r];
+                } else {
+                    *cluster.map_shared_rank(&sm.pair[to % span], to / span) = make_uint2(key[r], pos[r]);
+                }
             }
-        __syncthreads();
+        cluster.sync();   // the pairs have arrived, and nobody reads this CTA's counts any more
+        if (!last) {
 #pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r)
-            if (r < rounds && first + r * 32 < n) {
-                key[r] = sm.key[first + r * 32];
-                pos[r] = sm.pos[first + r * 32];
-            }
+            for (int r = 0; r < ROUNDS; ++r)
+                if (live[r]) {
+                    const uint2 v = sm.pair[local + r * 32];
+                    key[r] = v.x;
+                    pos[r] = v.y;
+                }
+        }
     }
-#pragma unroll
-    for (int r = 0; r < kSmallRounds; ++r)
-        if (r < rounds && first + r * 32 < n) {
-            p.key_out[first + r * 32] = key[r];
-            p.pos_out[first + r * 32] = pos[r];
-        }
-    if (threadIdx.x == 0) *p.joins = 0;
+    if (me == 0 && threadIdx.x == 0) *p.joins = 0;
+}
+
+constexpr long long kZeroBase = 30, kZeroPerRound = 12;   // MB cleared beside a sort of so many rounds
+
+template <typename I, int ROUNDS>
+static cudaError_t sort_cluster(const SortParams& p, int passes, int digit_bits, int ctas, cudaStream_t s) {
+    auto k = sort_cluster_kernel<I, ROUNDS>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared<ROUNDS>));
+    if (e == cudaSuccess && ctas > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    // clusters that clear, each CTA at least 64 KB: no more than find room beside the sort, a cluster to a GPC where it has sixteen CTAs
+    const long long want = p.zero_bytes / (65536ll * ctas) + (p.zero_bytes > 0), most = 96 / ctas;
+    cfg.gridDim = dim3(ctas * (unsigned)(1 + (want < most ? want : most)));
+    cfg.blockDim = dim3(kClusterThreads);
+    cfg.dynamicSmemBytes = sizeof(SortShared<ROUNDS>);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, p, passes, digit_bits);
 }
 
 // ---- sums over the sorted list ---------------------------------------------------------------------------
@@ -326,7 +389,8 @@ struct EmbGradParams {
     float* part;           // [chunks][2][cols]: a chunk's sum of an id that began before it, and of one that begins in it and is joined
     uint32_t* joins;       // how many ids are joined, and the chunks where they begin
     long long n, vocab, cols, chunks;
-    int zero_blocks;       // the first blocks zero, the others add
+    long long zero_rows;   // of these rows those that no id names are still to be cleared, the rest is
+    int zero_blocks;       // the first blocks clear, the others add
     float scale;
     int accumulate;
     int tiles;             // column tiles of a row
@@ -382,13 +446,14 @@ struct EmbLane {
     }
 };
 
+constexpr int kZeroRows = 8;   // of a warp at a time
 // Table rows that no id names: a lane looks one row up in the sorted list, the warp zeroes those that are missing.
 template <typename G, bool VEC>
 __device__ __forceinline__ void emb_zero(const EmbGradParams& p, int lane, int warp) {
-    const long long step = (long long)p.zero_blocks * 8 * 32;
-    for (long long r0 = ((long long)blockIdx.x * 8 + warp) * 32; r0 < p.vocab; r0 += step) {
+    const long long step = (long long)p.zero_blocks * 8 * kZeroRows;
+    for (long long r0 = ((long long)blockIdx.x * 8 + warp) * kZeroRows; r0 < p.zero_rows; r0 += step) {
         bool missing = false;
-        if (r0 + lane < p.vocab) {
+        if (lane < kZeroRows && r0 + lane < p.zero_rows) {
             const uint32_t v = (uint32_t)(r0 + lane);
             long long lo = 0, hi = p.n;
             while (lo < hi) {
@@ -659,7 +724,8 @@ static EmbWorkspace emb_workspace(long long n, long long vocab, long long cols) 
 }
 
 template <typename I>
-static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long n, long long vocab, long long padding, int* result, cudaStream_t s) {
+static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long n, long long vocab, long long padding, void* dtable,
+                    long long row_bytes, long long* zero_rows, int* result, cudaStream_t s) {
     SortParams p{};
     p.ids = ids;
     p.n = n;
@@ -668,13 +734,26 @@ static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long 
     p.tiles = w.tiles;
     p.bins = 1 << w.digit_bits;
     p.joins = reinterpret_cast<uint32_t*>(ws + w.joins);
-    if (n <= kSortSmall) {
+    constexpr int kRound = kClusterThreads;   // pairs of a round of one CTA
+    if (n <= 16 * 8 * kRound) {
+        // as many CTAs as have a round to do, then as few rounds as sixteen CTAs leave
         p.key_out = reinterpret_cast<uint32_t*>(ws + w.key[0]);
         p.pos_out = reinterpret_cast<uint32_t*>(ws + w.pos[0]);
-        CGB_CUDA(cudaFuncSetAttribute(sort_small_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmall)));
-        sort_small_kernel<I><<<1, kSmallWarps * 32, sizeof(SortSmall), s>>>(p, w.passes, w.digit_bits);
-        CGB_CUDA(cudaGetLastError());
+        int ctas = 1, rounds = 1;
+        while (ctas < 16 && ctas * kRound < n) ctas *= 2;
+        while (rounds * ctas * kRound < n) rounds *= 2;
         *result = 0;
+        // rows to clear meanwhile: what memory takes in the time of the sort
+        const long long fit = ((kZeroBase + kZeroPerRound * rounds) << 20) / row_bytes, rows = fit < *zero_rows ? fit : *zero_rows;
+        *zero_rows -= rows;
+        p.zero_from = static_cast<char*>(dtable) + *zero_rows * row_bytes;
+        p.zero_bytes = rows * row_bytes;
+        switch (rounds) {
+            case 1: CGB_CUDA((sort_cluster<I, 1>(p, w.passes, w.digit_bits, ctas, s))); break;
+            case 2: CGB_CUDA((sort_cluster<I, 2>(p, w.passes, w.digit_bits, ctas, s))); break;
+            case 4: CGB_CUDA((sort_cluster<I, 4>(p, w.passes, w.digit_bits, ctas, s))); break;
+            default: CGB_CUDA((sort_cluster<I, 8>(p, w.passes, w.digit_bits, ctas, s)));
+        }
         return CG_B200_OK;
     }
     int cur = 0;
@@ -709,8 +788,8 @@ static int emb_backward(EmbGradParams p, cudaStream_t s) {
     const bool vec = p.cols % L == 0 && aligned_to(p.dout, 16) && aligned_to(p.dtable, 16);
     const long long per = vec ? 32 * L : 256;
     p.tiles = (int)((p.cols + per - 1) / per);
-    const long long zero_cap = (long long)sm_count() * 8, want = (p.vocab + 255) / 256;
-    p.zero_blocks = p.accumulate ? 0 : (int)(want < zero_cap ? want : zero_cap);
+    const long long zero_cap = (long long)sm_count() * 32, want = (p.zero_rows + 8 * kZeroRows - 1) / (8 * kZeroRows);
+    p.zero_blocks = (int)(want < zero_cap ? want : zero_cap);
     const long long blocks = (p.chunks * p.tiles + 7) / 8 + p.zero_blocks;
     if (blocks > 0x7fffffffll) return CG_B200_ERR_UNSUPPORTED;
     if (vec) {
@@ -789,9 +868,11 @@ extern "C" int cg_b200_embedding_backward(int dtype, int grad_dtype, const void*
     cudaStream_t s = (cudaStream_t)stream;
     char* ws = static_cast<char*>(workspace);
     int sorted = 0;
+    long long zero_rows = accumulate ? 0 : vocab;
     if (n > 0) {
-        st = id_bytes == 4 ? emb_sort<int32_t>(w, ws, ids, n, vocab, padding_id, &sorted, s)
-                           : emb_sort<int64_t>(w, ws, ids, n, vocab, padding_id, &sorted, s);
+        const long long row_bytes = cols * (long long)dtype_bytes(grad_dtype);
+        st = id_bytes == 4 ? emb_sort<int32_t>(w, ws, ids, n, vocab, padding_id, dtable, row_bytes, &zero_rows, &sorted, s)
+                           : emb_sort<int64_t>(w, ws, ids, n, vocab, padding_id, dtable, row_bytes, &zero_rows, &sorted, s);
         if (st) return st;
     }
     EmbGradParams p{};
@@ -807,6 +888,7 @@ extern "C" int cg_b200_embedding_backward(int dtype, int grad_dtype, const void*
     p.chunks = w.chunks;
     p.scale = scale;
     p.accumulate = accumulate;
+    p.zero_rows = zero_rows;
     switch (dtype) {
         case CG_B200_F32: return emb_backward<float, float>(p, s);
         case CG_B200_BF16: return grad_dtype == CG_B200_F32 ? emb_backward<__nv_bfloat16, float>(p, s) : emb_backward<__nv_bfloat16, __nv_bfloat16>(p, s);

@@ -279,7 +279,8 @@ def test_embedding_forward(ops, types, n, vocab, cols):
 
 
 GRAD_CASES = [(1, 1, 1), (2, 1, 5), (31, 7, 64), (32, 3, 100), (33, 2, 256), (200, 100000, 40), (2048, 600, 264), (2049, 1, 128),
-              (5000, 300, 1032), (9999, 1000, 33), (4100, 300000, 16), (70000, 50000, 24)]
+              (5000, 300, 1032), (9999, 1000, 33), (4100, 300000, 16), (20000, 90, 16), (40000, 3000, 20), (70000, 50000, 24),
+              (140000, 700, 12), (150000, 300000, 5)]
 
 
 @pytest.mark.parametrize("types", [("F32", "F32"), ("BF16", "BF16"), ("BF16", "F32"), ("F16", "F16"), ("F16", "F32")])
