@@ -14,6 +14,8 @@
 // the sums.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace cgb {
@@ -33,72 +35,137 @@ __device__ __forceinline__ bool emb_id(const void* ids, long long n, long long v
     return id >= 0 && id < vocab;
 }
 
-// A warp takes one token and up to 128 packets (four per lane, all requested before the first is used).
-template <typename T, typename TT, typename I>
-__global__ void __launch_bounds__(256) emb_fwd_vec_kernel(const __grid_constant__ EmbParams p, int segments) {
-    constexpr int L = Vec16<T>::N, M = Vec16<TT>::N, R = L / M, U = 4;   // R table packets make one output packet
-    const int lane = threadIdx.x & 31;
-    const int packets = (int)(p.cols / L);
-    const long long units = p.n * segments, step = (long long)gridDim.x * 8;
+// Words `by` .. `by` + OUT - 1 of w, by < 4 (zero where w has no more)
+template <int OUT, int IN>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[IN], int by) {
+#pragma unroll
+    for (int i = 0; i < OUT + 1 && i < IN; ++i) w[i] = by & 2 ? (i + 2 < IN ? w[i + 2 < IN ? i + 2 : 0] : 0u) : w[i];
+#pragma unroll
+    for (int i = 0; i < OUT && i < IN; ++i) w[i] = by & 1 ? (i + 1 < IN ? w[i + 1 < IN ? i + 1 : 0] : 0u) : w[i];
+}
+
+// A warp takes TOK tokens and STEPS * 32 packets of their rows and requests all of them before it uses the first. (A flat walk over the
+// output's packets, with a division per packet, took 37 us instead of 28 for 65536 rows of 1024 bf16.)
+// RAGGED: the packets are the output's, whose rows start anywhere between 16-byte boundaries; a packet's columns lie in the table between
+// two other boundaries, `shift` elements on, the same for all packets of a row. So one aligned table packet more is read (L1 has it: it
+// is the next lane's) and the columns are shifted out of the words. Element loads and stores took 31 us for 30000 rows of 777 bf16.
+template <typename T, typename TT, typename I, bool RAGGED, int TOK, int STEPS>
+__global__ void __launch_bounds__(256) emb_fwd_kernel(const __grid_constant__ EmbParams p, int segments) {
+    constexpr int L = Vec16<T>::N, M = Vec16<TT>::N, R = L / M, MORE = RAGGED ? 1 : 0;   // R table packets make one output packet
+    const int lane = threadIdx.x & 31, cols = (int)p.cols;
+    const long long units = (p.n + TOK - 1) / TOK * segments, step = (long long)gridDim.x * 8;
+    const TT* const table = static_cast<const TT*>(p.table);
     for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += step) {
-        const long long n = u / segments;
-        const int k0 = (int)(u - n * segments) * (32 * U) + lane;
-        long long id;
-        const bool ok = emb_id<I>(p.ids, n, p.vocab, id);
-        const TT* src = static_cast<const TT*>(p.table) + (ok ? id : 0) * p.cols;
-        T* dst = static_cast<T*>(p.out) + n * p.cols;
-        Vec16<TT> v[U][R];
+        const long long n0 = segments == 1 ? u : u / segments;
+        const int k0 = (int)(u - n0 * segments) * (32 * STEPS) + lane;
+        Vec16<TT> v[TOK][STEPS][R + MORE];
+        bool ok[TOK];
+        int off[TOK], shift[TOK];
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-            if (ok && k0 + j * 32 < packets) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) v[j][r] = ld_keep(src + (long long)(k0 + j * 32) * L + r * M);
+        for (int t = 0; t < TOK; ++t) {
+            long long id = 0;
+            ok[t] = n0 * TOK + t < p.n && emb_id<I>(p.ids, n0 * TOK + t, p.vocab, id);
+            off[t] = shift[t] = 0;
+            const TT* row = table + id * p.cols;
+            if (RAGGED) {
+                off[t] = (int)((reinterpret_cast<uintptr_t>(static_cast<T*>(p.out) + (n0 * TOK + t) * p.cols) & 15) / sizeof(T));
+                shift[t] = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(TT) - off[t]) & (M - 1));
             }
+            const int lead = off[t] + shift[t];   // packet k begins `lead` columns before column k * L of the row
+            const TT* src = row + (k0 * L - lead);
+            // a row far enough from the table's ends is read in whole packets, with what lies beside it
+            if (!RAGGED || (id * p.cols >= L + M && (p.vocab - id) * p.cols >= p.cols + 2 * L + M)) {
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-            if (k0 + j * 32 < packets) {
-                float f[L];
+                for (int j = 0; j < STEPS; ++j)
+                    if (ok[t] && (k0 + j * 32) * L < off[t] + cols) {
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float t[M];
-                    unpack16<TT>(v[j][r], t);
+                        for (int r = 0; r < R + MORE; ++r) v[t][j][r] = ld_keep(src + j * 32 * L + r * M);
+                    }
+            } else {   // (id 0 is often the most frequent one: its first packet only is read by elements)
 #pragma unroll
-                    for (int i = 0; i < M; ++i) f[r * M + i] = ok ? t[i] * p.scale : 0.0f;
+                for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+                    for (int r = 0; r < R + MORE; ++r) {
+                        const int c0 = (k0 + j * 32) * L - lead + r * M;
+                        const long long at = id * p.cols + c0;
+                        if (ok[t] && c0 < cols && at >= 0 && at + M <= p.vocab * p.cols) {
+                            v[t][j][r] = ld_keep(row + c0);
+                        } else {
+#pragma unroll
+                            for (int l = 0; l < M; ++l)
+                                v[t][j][r].v[l] = ok[t] && c0 + l >= 0 && c0 + l < cols ? row[c0 + l] : Elem<TT>::from_f32(0.0f);
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TOK; ++t) {
+            if (n0 * TOK + t >= p.n) break;
+            T* dst = static_cast<T*>(p.out) + (n0 * TOK + t) * p.cols + (k0 * L - off[t]);
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                const int c0 = (k0 + j * 32) * L - off[t];
+                if (c0 < cols) {
+                    Vec16<TT> in[R];
+                    if constexpr (RAGGED) {
+                        uint32_t w[(R + 1) * 4];
+#pragma unroll
+                        for (int i = 0; i < (R + 1) * 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(&v[t][j][i / 4])[i % 4];
+                        if constexpr (sizeof(TT) == 4) {
+                            shift_words<R * 4>(w, shift[t]);
+                        } else {   // two elements to a word: words first, then half a word
+                            shift_words<5>(w, shift[t] >> 1);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16 * (shift[t] & 1));
+                        }
+#pragma unroll
+                        for (int i = 0; i < R * 4; ++i) reinterpret_cast<uint32_t*>(&in[i / 4])[i % 4] = w[i];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < R; ++r) in[r] = v[t][j][r];
+                    }
+                    float f[L];
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        float q[M];
+                        unpack16<TT>(in[r], q);
+#pragma unroll
+                        for (int i = 0; i < M; ++i) f[r * M + i] = ok[t] ? q[i] * p.scale : 0.0f;
+                    }
+                    const Vec16<T> o = pack16<T>(f);
+                    if (!RAGGED || (c0 >= 0 && c0 + L <= cols)) {
+                        st_stream(dst + j * 32 * L, o);
+                    } else {
+#pragma unroll
+                        for (int l = 0; l < L; ++l)
+                            if (c0 + l >= 0 && c0 + l < cols) dst[j * 32 * L + l] = o.v[l];
+                    }
                 }
-                st_stream(dst + (long long)(k0 + j * 32) * L, pack16<T>(f));
             }
+        }
     }
 }
 
-// Any width and alignment: a warp takes one token and up to 256 elements.
-template <typename T, typename TT, typename I>
-__global__ void __launch_bounds__(256) emb_fwd_scalar_kernel(const __grid_constant__ EmbParams p, long long segments) {
-    constexpr int U = 8;
-    const int lane = threadIdx.x & 31;
-    const long long units = p.n * segments, step = (long long)gridDim.x * 8;
-    for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += step) {
-        const long long n = u / segments, c0 = (u - n * segments) * (32 * U) + lane;
-        long long id;
-        const bool ok = emb_id<I>(p.ids, n, p.vocab, id);
-        const TT* src = static_cast<const TT*>(p.table) + (ok ? id : 0) * p.cols;
-        T* dst = static_cast<T*>(p.out) + n * p.cols;
-        float f[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) f[j] = ok && c0 + j * 32 < p.cols ? Elem<TT>::to_f32(src[c0 + j * 32]) * p.scale : 0.0f;
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-            if (c0 + j * 32 < p.cols) dst[c0 + j * 32] = Elem<T>::from_f32(f[j]);
-    }
+template <typename T, typename TT, typename I, bool RAGGED, int TOK, int STEPS>
+static void emb_forward_go(const EmbParams& p, long long per_row, cudaStream_t s) {
+    const long long segments = (per_row + 32 * STEPS - 1) / (32 * STEPS);
+    const long long blocks = ((p.n + TOK - 1) / TOK * segments + 7) / 8, cap = 1ll << 30;
+    emb_fwd_kernel<T, TT, I, RAGGED, TOK, STEPS><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, s>>>(p, (int)segments);
 }
 
 template <typename T, typename TT, typename I>
 static int emb_forward(const EmbParams& p, cudaStream_t s) {
-    const bool vec = p.cols % Vec16<T>::N == 0 && p.cols < (1ll << 30) && aligned_to(p.table, 16) && aligned_to(p.out, 16);
-    const long long per = vec ? 128 * Vec16<T>::N : 256, segments = (p.cols + per - 1) / per;
-    const long long blocks = (p.n * segments + 7) / 8, cap = 1ll << 30;
-    const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
-    if (vec) emb_fwd_vec_kernel<T, TT, I><<<grid, 256, 0, s>>>(p, (int)segments);
-    else emb_fwd_scalar_kernel<T, TT, I><<<grid, 256, 0, s>>>(p, segments);
+    constexpr int L = Vec16<T>::N;
+    const bool ragged = p.cols % L != 0 || !aligned_to(p.table, 16) || !aligned_to(p.out, 16);
+    const long long per_row = ragged ? (p.cols + 2 * L - 2) / L : p.cols / L;   // packets of a row at most
+    // little work: less of it per warp, so that every SM has some
+    const bool few = p.n * ((per_row + 31) / 32) < (long long)sm_count() * 64;
+    if (ragged && few) emb_forward_go<T, TT, I, true, 1, 1>(p, per_row, s);
+    else if (ragged) emb_forward_go<T, TT, I, true, 1, 4>(p, per_row, s);
+    else if (few) emb_forward_go<T, TT, I, false, 1, 1>(p, per_row, s);
+    else if (per_row <= 32) emb_forward_go<T, TT, I, false, 4, 1>(p, per_row, s);
+    else if (per_row <= 64) emb_forward_go<T, TT, I, false, 2, 2>(p, per_row, s);
+    else emb_forward_go<T, TT, I, false, 1, 4>(p, per_row, s);
     CGB_CUDA(cudaGetLastError());
     return CG_B200_OK;
 }
@@ -128,7 +195,7 @@ struct SortParams {
 __device__ __forceinline__ void zero_range(char* from, long long bytes, long long at, long long of) {
     const long long to_edge = (16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15, head = to_edge < bytes ? to_edge : bytes;
     const long long packets = (bytes - head) / 16;
-    if (at < head) from[at] = 0;
+    for (long long i = at; i < head; i += of) from[i] = 0;
     for (long long i = head + packets * 16 + at; i < bytes; i += of) from[i] = 0;
     int4* body = reinterpret_cast<int4*>(from + head);
     for (long long i = at; i < packets; i += of) __stcs(body + i, make_int4(0, 0, 0, 0));
@@ -448,7 +515,7 @@ struct EmbLane {
 
 constexpr int kZeroRows = 8;   // of a warp at a time
 // Table rows that no id names: a lane looks one row up in the sorted list, the warp zeroes those that are missing.
-template <typename G, bool VEC>
+template <typename G>
 __device__ __forceinline__ void emb_zero(const EmbGradParams& p, int lane, int warp) {
     const long long step = (long long)p.zero_blocks * 8 * kZeroRows;
     for (long long r0 = ((long long)blockIdx.x * 8 + warp) * kZeroRows; r0 < p.zero_rows; r0 += step) {
@@ -467,12 +534,7 @@ __device__ __forceinline__ void emb_zero(const EmbGradParams& p, int lane, int w
         while (todo) {
             const long long row = r0 + __ffs(todo) - 1;
             todo &= todo - 1;
-            G* dst = static_cast<G*>(p.dtable) + row * p.cols;
-            if constexpr (VEC) {
-                for (long long k = lane; k < p.cols / Vec16<G>::N; k += 32) __stcs(reinterpret_cast<int4*>(dst) + k, make_int4(0, 0, 0, 0));
-            } else {
-                for (long long c = lane; c < p.cols; c += 32) dst[c] = Elem<G>::from_f32(0.0f);
-            }
+            zero_range(reinterpret_cast<char*>(static_cast<G*>(p.dtable) + row * p.cols), p.cols * (long long)sizeof(G), lane, 32);
         }
     }
 }
@@ -519,16 +581,18 @@ __device__ __forceinline__ EmbSpan emb_span(const EmbGradParams& p, long long ch
 }
 
 // The rows come through shared memory, sixteen of a warp's 512-byte pieces under way at a time: requested as register loads they would
-// either cost the registers of as many packets or be waited for one by one (86 us instead of {GRAD_US} us for 57344 rows of 1024 bf16).
+// either cost the registers of as many packets or be waited for one by one (86 us instead of 45 for 57344 rows of 1024 bf16).
+// VEC: a lane owns the columns of one store of the table's type (or two). Otherwise, for widths that no packet divides, a row's piece is
+// copied as the packets that cover it, one more than it fills, and a lane owns every 32nd column and finds it behind the row's own offset.
 constexpr int kEmbRows = 4, kEmbGroups = 4;   // rows of a copy group, groups in flight
-template <typename T, typename G>
+template <typename T, typename G, bool VEC>
 __global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant__ EmbGradParams p) {
-    constexpr int L = Vec16<T>::N, E = Vec16<G>::N < L ? Vec16<G>::N : L, NP = L / E;
+    constexpr int L = Vec16<T>::N, E = !VEC ? 1 : Vec16<G>::N < L ? Vec16<G>::N : L, NP = L / E, SLOT = VEC ? 32 : 33;
     extern __shared__ float4 emb_smem4[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_trigger();
     pdl_wait();
-    if (blockIdx.x < p.zero_blocks) return emb_zero<G, true>(p, lane, warp);
+    if (blockIdx.x < p.zero_blocks) return emb_zero<G>(p, lane, warp);
     const long long unit = (long long)(blockIdx.x - p.zero_blocks) * 8 + warp;
     const long long chunk = unit / p.tiles;
     if (chunk >= p.chunks) return;
@@ -536,16 +600,30 @@ __global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant_
     const EmbSpan span = emb_span(p, chunk, lane);
     if (span.begin >= span.end) return;
     if (span.slot == 1 && tile0 == 0 && lane == 0) p.joins[1 + atomicAdd(p.joins, 1u)] = (uint32_t)chunk;   // in any order: each is joined by itself
-    // a warp's ring: [groups][rows][32 packets]; lane l copies packet l of a row and reads the pieces of its own columns
-    Vec16<T>* ring = reinterpret_cast<Vec16<T>*>(emb_smem4) + warp * (kEmbGroups * kEmbRows * 32);
-    const T* src = static_cast<const T*>(p.dout) + tile0 + lane * L;
-    const bool in = tile0 + lane * L < p.cols;   // whole packets: cols is a multiple of L
+    // a warp's ring: [groups][rows][SLOT packets]
+    Vec16<T>* ring = reinterpret_cast<Vec16<T>*>(emb_smem4) + warp * (kEmbGroups * kEmbRows * SLOT);
+    const T* const dout = static_cast<const T*>(p.dout);
+    const int width = (int)(p.cols - tile0 < 32 * L ? p.cols - tile0 : 32 * L);
+    auto offset = [&](long long pos) { return VEC ? 0 : (int)((reinterpret_cast<uintptr_t>(dout + pos * p.cols + tile0) & 15) / sizeof(T)); };
     auto fetch = [&](int group, int i) {   // rows i .. of the span into group `group`
 #pragma unroll
         for (int r = 0; r < kEmbRows; ++r)
             if (i + r < span.end) {
-                const T* from = src + (long long)span.at(i + r) * p.cols;
-                if (in) copy16_async(ring + (group * kEmbRows + r) * 32 + lane, from);
+                const long long pos = span.at(i + r);
+                const int off = offset(pos);
+                const T* from = dout + pos * p.cols + tile0 - off;
+                Vec16<T>* to = ring + (group * kEmbRows + r) * SLOT;
+                for (int k = lane; k * L < off + width; k += 32) {
+                    const T* src = from + k * L;
+                    if (VEC || (src >= dout && src + L <= dout + p.n * p.cols)) {
+                        copy16_async(to + k, src);
+                    } else {   // the packets at the tensor's ends: only what is inside
+                        Vec16<T> v;
+#pragma unroll
+                        for (int l = 0; l < L; ++l) v.v[l] = src + l >= dout && src + l < dout + p.n * p.cols ? src[l] : Elem<T>::from_f32(0.0f);
+                        to[k] = v;
+                    }
+                }
             }
         copy_commit();
     };
@@ -570,68 +648,25 @@ __global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant_
                 cur = id;
                 acc.clear();
             }
-            const T* row = reinterpret_cast<const T*>(ring + (group * kEmbRows + r) * 32);
+            const T* row = reinterpret_cast<const T*>(ring + (group * kEmbRows + r) * SLOT) + (VEC ? 0 : offset(span.at(i0 + r))) + lane * E;
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
-                Vec16<T> v;
-                if constexpr (NP == 1) v = *reinterpret_cast<const Vec16<T>*>(row + lane * E);
-                else *reinterpret_cast<int2*>(&v) = *reinterpret_cast<const int2*>(row + q * 32 * E + lane * E);   // half a packet
-                float t[L];
-                unpack16<T>(v, t);
+                if constexpr (E == 1) {
+                    acc.v[q][0] += Elem<T>::to_f32(row[q * 32]);   // (behind the row's end: what is there, added to a column that is not written)
+                } else {
+                    Vec16<T> v;
+                    if constexpr (NP == 1) v = *reinterpret_cast<const Vec16<T>*>(row);
+                    else *reinterpret_cast<int2*>(&v) = *reinterpret_cast<const int2*>(row + q * 32 * E);   // half a packet
+                    float t[L];
+                    unpack16<T>(v, t);
 #pragma unroll
-                for (int l = 0; l < E; ++l) acc.v[q][l] += t[l];
+                    for (int l = 0; l < E; ++l) acc.v[q][l] += t[l];
+                }
             }
         }
         __syncwarp();
         fetch(group, i0 + kEmbGroups * kEmbRows);
         group = group + 1 == kEmbGroups ? 0 : group + 1;
-    }
-    if (head_part) acc.write_part(p, chunk, 0, c0);
-    else if (span.slot >= 0) acc.write_part(p, chunk, span.slot, c0);
-    else acc.write(p, cur, c0);
-}
-
-// Any width and alignment: a lane owns eight columns, 32 apart, and reads them one by one.
-template <typename T, typename G>
-__global__ void __launch_bounds__(256) emb_grad_scalar_kernel(const __grid_constant__ EmbGradParams p) {
-    constexpr int NP = 8, U = 4;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_trigger();
-    pdl_wait();
-    if (blockIdx.x < p.zero_blocks) return emb_zero<G, false>(p, lane, warp);
-    const long long unit = (long long)(blockIdx.x - p.zero_blocks) * 8 + warp;
-    const long long chunk = unit / p.tiles;
-    if (chunk >= p.chunks) return;
-    const long long c0 = (unit - chunk * p.tiles) * (32 * NP) + lane;
-    const EmbSpan span = emb_span(p, chunk, lane);
-    if (span.begin >= span.end) return;
-    if (span.slot == 1 && c0 == 0) p.joins[1 + atomicAdd(p.joins, 1u)] = (uint32_t)chunk;
-    EmbLane<G, 1, NP> acc;
-    acc.clear();
-    uint32_t cur = span.id(span.begin);
-    bool head_part = span.head_part;
-    for (int i0 = span.begin; i0 < span.end; i0 += U) {
-        float v[U][NP];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const T* src = static_cast<const T*>(p.dout) + (long long)span.at(i0 + u) * p.cols + c0;
-#pragma unroll
-            for (int q = 0; q < NP; ++q) v[u][q] = i0 + u < span.end && c0 + q * 32 < p.cols ? Elem<T>::to_f32(src[q * 32]) : 0.0f;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u >= span.end) break;
-            const uint32_t id = span.id(i0 + u);
-            if (id != cur) {
-                if (head_part) acc.write_part(p, chunk, 0, c0);
-                else acc.write(p, cur, c0);
-                head_part = false;
-                cur = id;
-                acc.clear();
-            }
-#pragma unroll
-            for (int q = 0; q < NP; ++q) acc.v[q][0] += v[u][q];
-        }
     }
     if (head_part) acc.write_part(p, chunk, 0, c0);
     else if (span.slot >= 0) acc.write_part(p, chunk, span.slot, c0);
@@ -786,18 +821,16 @@ template <typename T, typename G>
 static int emb_backward(EmbGradParams p, cudaStream_t s) {
     constexpr int L = Vec16<T>::N;
     const bool vec = p.cols % L == 0 && aligned_to(p.dout, 16) && aligned_to(p.dtable, 16);
-    const long long per = vec ? 32 * L : 256;
-    p.tiles = (int)((p.cols + per - 1) / per);
+    p.tiles = (int)((p.cols + 32 * L - 1) / (32 * L));
     const long long zero_cap = (long long)sm_count() * 32, want = (p.zero_rows + 8 * kZeroRows - 1) / (8 * kZeroRows);
     p.zero_blocks = (int)(want < zero_cap ? want : zero_cap);
     const long long blocks = (p.chunks * p.tiles + 7) / 8 + p.zero_blocks;
     if (blocks > 0x7fffffffll) return CG_B200_ERR_UNSUPPORTED;
-    if (vec) {
-        constexpr int smem = 8 * kEmbGroups * kEmbRows * 512;
-        CGB_CUDA(cudaFuncSetAttribute(emb_grad_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        CGB_CUDA(launch_pdl(emb_grad_kernel<T, G>, (unsigned)blocks, 256, smem, s, p));
-    } else {
-        CGB_CUDA(launch_pdl(emb_grad_scalar_kernel<T, G>, (unsigned)blocks, 256, 0, s, p));
+    auto k = vec ? emb_grad_kernel<T, G, true> : emb_grad_kernel<T, G, false>;
+    const int smem = 8 * kEmbGroups * kEmbRows * (vec ? 32 : 33) * 16;
+    if (blocks > 0) {
+        CGB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CGB_CUDA(launch_pdl(k, (unsigned)blocks, 256, smem, s, p));
     }
     if (p.n > kChunk) {   // fewer cannot cover a chunk and reach beyond it
         const int e = p.cols % 4 == 0 ? 4 : 1;
@@ -808,7 +841,7 @@ static int emb_backward(EmbGradParams p, cudaStream_t s) {
 }
 
 static bool emb_sizes_ok(int64_t n, int64_t vocab, int64_t cols) {
-    return n >= 0 && vocab >= 0 && cols >= 0 && n <= 0x7fffffff && vocab < 0x7fffffff && cols <= 0x7fffffff;
+    return n >= 0 && vocab >= 0 && cols >= 0 && n <= 0x7fffffff && vocab < 0x7fffffff && cols <= (1 << 30);
 }
 
 }  // namespace cgb
