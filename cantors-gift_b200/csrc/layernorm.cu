@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
     const int tpr = SUB ? 8 : sh.tpr, group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr, warps = tpr >> 5;
     LnSums<2 * R>* scratch = scratch_all + (SUB ? 0 : group * 32);
     int phase = 0;
+    pdl_trigger();
     const int cols = (int)p.cols;
     const int off = RAGGED ? (int)((p.off0 + (long long)blockIdx.x * cols) % L) : 0;
     const int n_pkt = (off + cols + L - 1) / L;
@@ -645,6 +646,8 @@ __global__ void __launch_bounds__(256) ln_bwd_columns_kernel(const __grid_consta
 template <typename TP>
 __global__ void __launch_bounds__(512) ln_weight_grad_kernel(const float* part, long long parts, long long cols, TP* dgamma, TP* dbeta) {
     __shared__ float sum[16][32];
+    pdl_trigger();
+    pdl_wait();
     TP* out = blockIdx.y ? dbeta : dgamma;
     const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
     float s = 0.0f;
@@ -758,9 +761,8 @@ static int ln_backward(const LnParams& p, void* dgamma, void* dbeta, cudaStream_
         }
     }
     if (dgamma || dbeta) {
-        ln_weight_grad_kernel<TP><<<dim3((unsigned)((p.cols + 31) / 32), 2), dim3(32, 16), 0, s>>>(p.part, parts, p.cols, static_cast<TP*>(dgamma),
-                                                                                                  static_cast<TP*>(dbeta));
-        CGB_CUDA(cudaGetLastError());
+        CGB_CUDA(launch_pdl(ln_weight_grad_kernel<TP>, dim3((unsigned)((p.cols + 31) / 32), 2), dim3(32, 16), 0, s, (const float*)p.part,
+                            (long long)parts, p.cols, static_cast<TP*>(dgamma), static_cast<TP*>(dbeta)));
     }
     return CG_B200_OK;
 }
