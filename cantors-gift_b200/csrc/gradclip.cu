@@ -6,8 +6,8 @@
 //
 // HBM-bound: the list is read for the norm and again for the scaling, which cannot begin before the norm is known, and written once.
 // The tensors' addresses, lengths and types travel by value in the kernel's parameters, so nothing is copied to the device first and
-// nothing is kept between calls. Each tensor is cut into chunks and the CTAs walk the chunks of all tensors gridDim.x apart; squares are added in fp32 per 16-byte packet and in fp64 beyond it, and every CTA leaves one fp64 sum in the
-// workspace. The scaling kernel's CTAs each add those sums up in the same fixed order, so the norm does not depend on timing, and walk
+// nothing is kept between calls. The list is cut into as many equal pieces as there are CTAs; squares are added in fp32 per 16-byte packet
+// and in fp64 beyond it, and every CTA leaves one fp64 sum in the workspace. The scaling kernel's CTAs each add those sums up in the same fixed order, so the norm does not depend on timing, and walk
 // their pieces backwards: what the norm pass read last is still in L2.
 #include <float.h>
 #include <stdlib.h>
@@ -23,7 +23,9 @@ namespace cgb {
 // parameters and 5 us with 400), a long one up to the parameter limit for the others.
 constexpr int kClipShort = 64, kClipLong = 448;
 constexpr int kClipChunk = 2048;   // elements; what a CTA takes is a run of chunks
-constexpr int kClipThreads = 256;
+// Many threads with two requests each: 56 us for 34M bf16 gradients into fp32, against 57 with four requests and half the threads and 59
+// with eight and three eighths.
+constexpr int kClipThreads = 256, kClipCtas = 8;   // of a CTA; CTAs of an SM
 
 struct ClipEntry {
     const void* in;
@@ -86,7 +88,7 @@ __device__ __forceinline__ double clip_squares(const Vec16<T>& v) {
 
 template <typename T>
 __device__ __forceinline__ double clip_run_squares(const T* g, long long n) {
-    constexpr int L = Vec16<T>::N, U = 4;
+    constexpr int L = Vec16<T>::N, U = 2;
     const long long head = clip_head(g, n), packets = (n - head) / L;
     double sum = 0.0;
     for (long long i = threadIdx.x; i < head; i += kClipThreads) sum += (double)Elem<T>::to_f32(g[i]) * (double)Elem<T>::to_f32(g[i]);
@@ -117,7 +119,7 @@ __device__ __forceinline__ double clip_block_sum(double v, double* scratch) {
 }
 
 template <int N>
-__global__ void __launch_bounds__(kClipThreads, 4) clip_norm_kernel(const __grid_constant__ ClipTable<N> t) {
+__global__ void __launch_bounds__(kClipThreads, kClipCtas) clip_norm_kernel(const __grid_constant__ ClipTable<N> t) {
     __shared__ double scratch[kClipThreads / 32];
     double sum = 0.0;
     pdl_trigger();
@@ -145,7 +147,7 @@ __device__ __forceinline__ double clip_norm(const double* parts, int n, double* 
 // read 8 bytes at a time.
 template <typename T, typename O>
 __device__ __forceinline__ void clip_run_scale(const T* g, O* o, long long n, float factor) {
-    constexpr int E = Vec16<O>::N, U = 4;   // elements of a piece; sizeof(O) >= sizeof(T)
+    constexpr int E = Vec16<O>::N, U = 2;   // elements of a piece; sizeof(O) >= sizeof(T)
     typedef typename std::conditional<E * sizeof(T) == 16, int4, int2>::type Raw;
     const long long head = clip_head(o, n);
     const bool vec = (reinterpret_cast<uintptr_t>(g + head) & (sizeof(Raw) - 1)) == 0;   // both sides reach a boundary at the same element
@@ -175,7 +177,7 @@ __device__ __forceinline__ void clip_run_scale(const T* g, O* o, long long n, fl
 }
 
 template <int N>
-__global__ void __launch_bounds__(kClipThreads, 4) clip_scale_kernel(const __grid_constant__ ClipTable<N> t) {
+__global__ void __launch_bounds__(kClipThreads, kClipCtas) clip_scale_kernel(const __grid_constant__ ClipTable<N> t) {
     __shared__ double scratch[kClipThreads / 32];
     pdl_trigger();
     pdl_wait();
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_only_kernel(const doub
     if (threadIdx.x == 0) *norm = (float)v;
 }
 
-static long long clip_grid_cap() { return (long long)sm_count() * 4; }
+static long long clip_grid_cap() { return (long long)sm_count() * kClipCtas; }
 
 // Nothing may be written twice, and nothing written may be another's input: a tensor is scaled in place, or into memory of its own. The
 // address ranges are sorted and swept once.
