@@ -45,7 +45,7 @@ constexpr int kLnWarps = kLnThreads / 32;
 
 // Sums of N values over the threads that share a row (8 lanes of a warp when SUB, else `warps` warps); every thread gets them. The warps
 // of a group meet at barrier `bar`; two scratch halves take turns, so one barrier per call is enough.
-template <int N> struct alignas(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) LnSums {
+template <int N> struct alignas(N % 2 == 0 ? 8 : 4) LnSums {
     float v[N];
 };
 template <int N>
@@ -85,6 +85,44 @@ __device__ __forceinline__ void row_sum(LnSums<N>& s, LnSums<N>* scratch, int& p
 #pragma unroll
         for (int i = 0; i < N; ++i) s.v[i] = __shfl_sync(0xffffffffu, s.v[i], 0);
     }
+}
+
+// The same for two values, which is what the kernels below reduce, with half the shuffles: from the first exchange on, one half of the lanes
+// adds up the first value and the other half the second. Behind the barrier every thread reads all warps' sums, two to a 16-byte read;
+// entries from `warps` on are zero (row_sum2_prepare).
+template <bool SUB>
+__device__ __forceinline__ void row_sum2(LnSums<2>& s, LnSums<2>* scratch, int& phase, int bar, int warps) {
+    constexpr int HALF = SUB ? 4 : 16;
+    const int lane = threadIdx.x & 31;
+    const unsigned mask = SUB ? 0xffu << (lane & 24) : 0xffffffffu;
+    const bool second = lane & HALF;
+    float v = second ? s.v[1] : s.v[0];
+    v += __shfl_xor_sync(mask, second ? s.v[0] : s.v[1], HALF);
+#pragma unroll
+    for (int o = HALF / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+    if (SUB || warps == 1) {
+        s.v[0] = __shfl_sync(mask, v, SUB ? lane & 24 : 0);
+        s.v[1] = __shfl_sync(mask, v, (SUB ? lane & 24 : 0) + HALF);
+        return;
+    }
+    LnSums<2>* at = scratch + phase;
+    phase ^= 16;
+    if ((lane & 15) == 0) at[(threadIdx.x >> 5) % warps].v[lane >> 4] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
+    const float4* q = reinterpret_cast<const float4*>(at);
+    auto two = [&](int i) {
+        const float4 t = q[i];
+        return __fadd2_rn(make_float2(t.x, t.y), make_float2(t.z, t.w));
+    };
+    float2 t = __fadd2_rn(two(0), two(1));
+    if (warps > 4) t = __fadd2_rn(t, __fadd2_rn(two(2), two(3)));
+    if (warps > 8) t = __fadd2_rn(t, __fadd2_rn(__fadd2_rn(two(4), two(5)), __fadd2_rn(two(6), two(7))));
+    s.v[0] = t.x;
+    s.v[1] = t.y;
+}
+// By all threads of a group, lane their number in it, before its first row_sum2
+__device__ __forceinline__ void row_sum2_prepare(LnSums<2>* scratch, int lane, int warps) {
+    if (lane < 32 && (lane & 15) >= warps) scratch[lane] = LnSums<2>{};
 }
 
 // until at most `stages` - 1 of this thread's groups are under way
@@ -214,11 +252,12 @@ template <typename T, typename TP, int CH, int R, bool SUB, bool RAGGED>
 __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_constant__ LnParams p, const LnShape sh) {
     constexpr int L = Vec16<T>::N;
     extern __shared__ float4 ln_smem4[];
-    __shared__ LnSums<R> scratch_all[SUB ? 1 : kLnWarps * 32];
+    __shared__ alignas(16) LnSums<R> scratch_all[SUB ? 1 : kLnWarps * 32];
     __shared__ uint4 keep_all[RAGGED ? kLnThreads / (SUB ? 8 : 32) * 2 : 1][RAGGED ? CH * L / 4 : 1];
     const int tpr = SUB ? 8 : sh.tpr, group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr, warps = tpr >> 5;
     LnSums<R>* scratch = scratch_all + (SUB ? 0 : group * 32);
     int phase = 0;
+    if constexpr (R == 2 && !SUB) row_sum2_prepare(scratch, lane, warps);
     const int cols = (int)p.cols;
     // all rows of this CTA share the offset of row blockIdx.x: gridDim.x is a multiple of L when rows are ragged
     const int off = RAGGED ? (int)((p.off0 + (long long)blockIdx.x * cols) % L) : 0;
@@ -291,7 +330,8 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
                 for (int l = 0; l < L / 2; ++l) t = __fadd2_rn(t, x[r][j][l]);
             s.v[r] = t.x + t.y;
         }
-        row_sum<SUB>(s, scratch, phase, group + 1, warps);
+        if constexpr (R == 2) row_sum2<SUB>(s, scratch, phase, group + 1, warps);
+        else row_sum<SUB>(s, scratch, phase, group + 1, warps);
         float mean[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -316,7 +356,8 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
                 for (int l = 0; l < L / 2; ++l) t = __ffma2_rn(x[r][j][l], x[r][j][l], t);
             s.v[r] = t.x + t.y;
         }
-        row_sum<SUB>(s, scratch, phase, group + 1, warps);
+        if constexpr (R == 2) row_sum2<SUB>(s, scratch, phase, group + 1, warps);
+        else row_sum<SUB>(s, scratch, phase, group + 1, warps);
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (r == 0 || i + r < left) {
@@ -356,12 +397,13 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
     constexpr bool KEEP = CH * L <= 16;
     static_assert(KEEP || R == 1, "rows at a time are kept in registers");
     extern __shared__ float4 ln_smem4[];
-    __shared__ LnSums<2 * R> scratch_all[SUB ? 1 : kLnWarps * 32];
+    __shared__ alignas(16) LnSums<2 * R> scratch_all[SUB ? 1 : kLnWarps * 32];
     __shared__ uint4 keep_all[RAGGED ? kLnThreads / (SUB ? 8 : 32) * 2 : 1][RAGGED ? CH * L / 4 : 1];
     const int tpr = SUB ? 8 : sh.tpr, group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr, warps = tpr >> 5;
     LnSums<2 * R>* scratch = scratch_all + (SUB ? 0 : group * 32);
     int phase = 0;
     pdl_trigger();
+    if constexpr (!SUB) row_sum2_prepare(scratch, lane, warps);
     const int cols = (int)p.cols;
     const int off = RAGGED ? (int)((p.off0 + (long long)blockIdx.x * cols) % L) : 0;
     const int n_pkt = (off + cols + L - 1) / L;
@@ -488,7 +530,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
             s.v[2 * r] = s1.x + s1.y;
             s.v[2 * r + 1] = s2.x + s2.y;
         }
-        row_sum<SUB>(s, scratch, phase, group + 1, warps);
+        row_sum2<SUB>(s, scratch, phase, group + 1, warps);
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (r == 0 || i + r < left) {
