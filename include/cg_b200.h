@@ -211,7 +211,7 @@ int cg_b200_softmax_layernorm(int dtype, const void* in, const void* gamma,
  * and sums are fp32, one rounding per result; the same inputs give the same bits on every call.
  * Forward: gamma, beta, mean, rstd may be NULL; in == out is allowed. Backward: gamma may be NULL (taken as 1); din,
  * dgamma, dbeta may each be NULL, not all three; din may be `dout` or `in` itself, not overlap them otherwise. rows == 0:
- * dgamma and dbeta become zero. The workspace (256-byte aligned, contents undefined before and after) is used only
+ * dgamma and dbeta become zero. The workspace (16-byte aligned, contents undefined before and after) is used only
  * when dgamma or dbeta is asked for; two calls that can run at the same time need one each. */
 int cg_b200_layernorm_forward(int dtype, int param_dtype, const void* in, const void* gamma, const void* beta, float eps,
                               void* out, float* mean, float* rstd, int64_t rows, int64_t cols, void* stream);

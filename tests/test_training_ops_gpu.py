@@ -101,7 +101,7 @@ def check_ln_backward(ops, dy, x, mean, rstd, gamma, dx=None, bias=True):
 # one column, fewer columns than a packet, widths on and beside every variant's border, widths that no packet divides, long rows
 LN_SHAPES = [(1, 1), (5, 3), (1, 8), (3, 64), (700, 64), (9, 65), (17, 100), (33, 256), (4, 257), (600, 512), (13, 513), (77, 1024),
              (1300, 1001), (2, 1025), (31, 2048), (6, 2047), (9, 4096), (40, 4099), (3, 8192), (5, 8200), (2, 16384), (3, 16385),
-             (2, 20001), (5000, 130)]
+             (2, 20001), (5000, 130), (7, 9001), (3, 16383), (1500, 72), (2000, 250), (301, 12001)]
 
 
 @pytest.mark.parametrize("params", ["own", "F32"])
@@ -570,3 +570,105 @@ def test_the_same_inputs_give_the_same_bits(ops):
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
         for a, b in zip(first[2], again[2]):
             assert torch.equal(a, b)
+
+
+def test_two_calls_at_once_on_two_streams(ops):
+    """The same operators on two streams, neither waiting for the other: each call has workspaces of its own."""
+    sets = [step_inputs(seed=21, n=(6000,), vocab=300, cols=513), step_inputs(seed=22, n=(9000,), vocab=40, cols=264)]
+    wants = [one_step(ops, *a, 1.0) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    gots = [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                gots[k].append(one_step(ops, *sets[k], 1.0))
+    torch.cuda.synchronize()
+    for (wy, wnorm, wgrads), got in zip(wants, gots):
+        for y, norm, grads in got:
+            assert torch.equal(y, wy) and torch.equal(norm, wnorm)
+            for a, b in zip(grads, wgrads):
+                assert torch.equal(a, b)
+
+
+def test_a_first_call_can_be_captured():
+    """The operators set nothing up that a capture would refuse: in a new process, the first call of each is a captured one."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = """
+import torch
+from cantors_gift_b200 import ops
+x = torch.randn(40, 300, device="cuda"); gamma = torch.randn(300, device="cuda")
+ids = torch.randint(0, 90, (40,), device="cuda"); table = torch.randn(90, 300, device="cuda")
+torch.cuda.synchronize()
+def step():
+    e = ops.embedding(table, ids)
+    y, m, r = ops.layernorm_forward(e, gamma, gamma)
+    dx, dg, db = ops.layernorm_backward(x, e, m, r, gamma)
+    dt = ops.embedding_backward(dx, ids, 90)
+    n = ops.grad_norm([dt, dg, db])
+    ops.clip_grad_norm([dt, dg, db], 0.5)
+    return y, dt, dg, db, n
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay(); torch.cuda.synchronize()
+for a, b in zip(out, step()):
+    assert torch.equal(a, b)
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+# ---- offsets that pass 32 bits ---------------------------------------------------------------------------------
+def test_layernorm_beyond_32_bit_offsets(ops):
+    """2.3e9 elements; all rows alike but the last three, which must come out as they do by themselves."""
+    rows, cols = 140001, 16384
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    x[:, ::2] = 1.0
+    tail = normal(3, cols, seed=1, dtype=torch.bfloat16)
+    x[-3:] = tail
+    gamma = normal(cols, seed=2)
+    y, mean, rstd = ops.layernorm_forward(x, gamma, gamma, out=torch.empty_like(x))
+    wy, wm, wr = ops.layernorm_forward(tail, gamma, gamma)
+    assert torch.equal(y[-3:], wy) and torch.equal(mean[-3:], wm) and torch.equal(rstd[-3:], wr)
+    assert torch.equal(y[0], y[rows // 2]) and float(mean[7]) == 0.5
+    dx, dg, db = ops.layernorm_backward(x, x, mean, rstd, gamma, dx=y)
+    wdx = ops.layernorm_backward(tail, tail, wm, wr, gamma)[0]
+    assert torch.equal(dx[-3:], wdx)
+    # dbeta: half of the columns add 1 in every row but the last three
+    want = (rows - 3) * (torch.arange(cols, device="cuda") % 2 == 0).double() + tail.double().sum(0)
+    assert_within(db, want, want.abs() + tail.double().abs().sum(0), "dbeta")
+
+
+def test_embedding_beyond_32_bit_offsets(ops):
+    vocab, cols = 1100000, 2048     # 2.25e9 elements
+    table = torch.zeros(vocab, cols, device="cuda", dtype=torch.bfloat16)
+    table[-2:] = normal(2, cols, seed=1, dtype=torch.bfloat16)
+    ids = torch.tensor([0, vocab - 1, vocab - 2, vocab], device="cuda")
+    out = ops.embedding(table, ids)
+    assert torch.equal(out[1], table[-1]) and torch.equal(out[2], table[-2]) and float(out[0].abs().max()) == 0 and float(out[3].abs().max()) == 0
+    dy = normal(4, cols, seed=2, dtype=torch.bfloat16)
+    grad = ops.embedding_backward(dy, ids, vocab, out=table)
+    assert torch.equal(grad[-1], dy[1]) and torch.equal(grad[-2], dy[2]) and torch.equal(grad[0], dy[0])
+    assert float(grad[1:-2].abs().amax()) == 0
+    del table, grad
+    n = 1100000
+    ids = torch.arange(n, device="cuda") % 7
+    dy = torch.ones(n, cols, device="cuda", dtype=torch.bfloat16)
+    grad = ops.embedding_backward(dy, ids, 9, dtype=torch.float32)
+    count = torch.bincount(ids, minlength=9).float()
+    assert torch.equal(grad, count[:, None].expand(9, cols))    # whole numbers below 2^24: exact in fp32
+    assert float(ops.embedding(grad.bfloat16(), ids, out=dy)[-1, -1]) == float(count[int(ids[-1])].bfloat16())
+
+
+def test_clip_beyond_32_bit_offsets(ops):
+    n = (1 << 31) + 1001
+    g = torch.full((n,), 2.0 ** -10, device="cuda", dtype=torch.bfloat16)
+    norm = ops.clip_grad_norm([g], 2.0)
+    want = (n * 2.0 ** -20) ** 0.5
+    assert abs(float(norm) - want) <= 6 * 2.0 ** -24 * want
+    value = torch.tensor(2.0 ** -10 * 2.0 / (want + 1e-6), dtype=torch.float64).to(torch.bfloat16)
+    assert float(g.min()) == float(value) == float(g.max())

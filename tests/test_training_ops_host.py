@@ -146,3 +146,31 @@ def test_python_entry_points_take_cuda_tensors(cgb):
         ops.clip_grad_norm([x], 1.0)
     with pytest.raises(ValueError):
         ops.grad_norm([])
+
+
+def test_calls_go_to_their_tensors_device(cgb, monkeypatch):
+    """A tensor on another device than the current one is worked on there, and a stream of a third one is refused (no GPU is touched)."""
+    import torch
+    from cantors_gift_b200 import ops
+
+    class Fake:
+        def __init__(self, index):
+            self.index, self.device = index, torch.device("cuda", index)
+
+        def get_device(self):
+            return self.index
+
+    class FakeStream:
+        def __init__(self, index):
+            self.device = torch.device("cuda", index)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: ("device", index))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: ("stream", s))
+    assert ops._elsewhere(Fake(0), None) is None
+    assert ops._elsewhere(Fake(1), None) == ("device", 1)
+    s = FakeStream(1)
+    assert ops._elsewhere(Fake(1), s) == ("stream", s)
+    with pytest.raises(ValueError):
+        ops._elsewhere(Fake(0), s)
