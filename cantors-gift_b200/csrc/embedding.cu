@@ -406,6 +406,19 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __g
                 const uint32_t digit = (key[r] >> shift) & low;
                 sm.local[sm.start[digit] + sm.cnt[warp][digit] + rank[r]] = make_uint2(key[r], pos[r]);
             }
+        const bool last = pass + 1 == passes;
+        if (ctas == 1) {   // `local` is the order of all
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r)
+                if (live[r]) {
+                    const uint2 v = sm.local[place + r * 32];
+                    key[r] = v.x;
+                    pos[r] = v.y;
+                    if (last) p.out[place + r * 32] = v;
+                }
+            continue;
+        }
         cluster.sync();   // every CTA's counts are there, and its pairs of the last pass have been taken out
         uint32_t total = 0, earlier = 0;
         if (bin)
@@ -418,7 +431,6 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __g
         const uint32_t before = bins_before(total, sm.warp_total, lane, warp);
         if (bin) sm.start[threadIdx.x] = before + earlier - start;   // from a pair's place in `local` to its place among all
         __syncthreads();
-        const bool last = pass + 1 == passes;
         for (int i = threadIdx.x; i < mine; i += kClusterThreads) {
             const uint2 v = sm.local[i];
             const uint32_t to = sm.start[(v.x >> shift) & low] + i;
