@@ -124,15 +124,22 @@ __global__ void __launch_bounds__(256) emb_fwd_kernel(const __grid_constant__ Em
 #pragma unroll
                         for (int r = 0; r < R; ++r) in[r] = v[t][j][r];
                     }
-                    float f[L];
+                    Vec16<T> o{};
+                    if (ok[t]) {   // the whole warp's token is, or is not
+                        float f[L];
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        float q[M];
-                        unpack16<TT>(in[r], q);
+                        for (int r = 0; r < R; ++r) {
+                            float q[M];
+                            unpack16<TT>(in[r], q);
 #pragma unroll
-                        for (int i = 0; i < M; ++i) f[r * M + i] = ok[t] ? q[i] * p.scale : 0.0f;
+                            for (int i = 0; i < M; i += 2) {
+                                const float2 v2 = __fmul2_rn(make_float2(q[i], q[i + 1]), make_float2(p.scale, p.scale));
+                                f[r * M + i] = v2.x;
+                                f[r * M + i + 1] = v2.y;
+                            }
+                        }
+                        o = pack16<T>(f);
                     }
-                    const Vec16<T> o = pack16<T>(f);
                     if (!RAGGED || (c0 >= 0 && c0 + L <= cols)) {
                         st_stream(dst + j * 32 * L, o);
                     } else {
@@ -571,6 +578,7 @@ __device__ __forceinline__ void emb_zero(const EmbGradParams& p, int lane, int w
 // What a warp does with its chunk: the pairs begin .. end - 1 of this chunk and the next one's are its own.
 struct EmbSpan {
     uint32_t key, pos, key2, pos2;   // lane l's pair of this chunk and of the next
+    unsigned long long change;       // bit i: pair i has another id than pair i - 1
     int begin, end;
     int slot;        // where the sum of the last id goes: -1 the table, 0 / 1 the workspace
     bool head_part;  // the first id's sum goes to the workspace (and it is not the last id)
@@ -590,6 +598,9 @@ __device__ __forceinline__ EmbSpan emb_span(const EmbGradParams& p, long long ch
     const uint32_t before = first > 0 ? p.pair[first - 1].x : none, before32 = first > 0 ? p.pair[first - kChunk].x : none;
     const uint32_t id0 = __shfl_sync(0xffffffffu, s.key, 0), id31 = __shfl_sync(0xffffffffu, s.key, 31);
     const uint32_t id32 = __shfl_sync(0xffffffffu, s.key2, 0), id63 = __shfl_sync(0xffffffffu, s.key2, 31);
+    const uint32_t left = __shfl_up_sync(0xffffffffu, s.key, 1), left2 = __shfl_up_sync(0xffffffffu, s.key2, 1);
+    s.change = __ballot_sync(0xffffffffu, lane > 0 && s.key != left) |
+               (unsigned long long)__ballot_sync(0xffffffffu, s.key2 != (lane > 0 ? left2 : id31)) << 32;
     s.begin = 0;
     s.end = __popc(__ballot_sync(0xffffffffu, s.key != none));   // dropped ids are last
     s.slot = -1;
@@ -635,23 +646,29 @@ __global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant_
     const T* const dout = static_cast<const T*>(p.dout);
     const int width = (int)(p.cols - tile0 < 32 * L ? p.cols - tile0 : 32 * L);
     auto offset = [&](long long pos) { return VEC ? 0 : (int)((reinterpret_cast<uintptr_t>(dout + pos * p.cols + tile0) & 15) / sizeof(T)); };
+    const T* const mine = dout + tile0 + lane * L;   // of row 0
+    const bool in = lane * L < width;
     auto fetch = [&](int group, int i) {   // rows i .. of the span into group `group`
 #pragma unroll
         for (int r = 0; r < kEmbRows; ++r)
             if (i + r < span.end) {
-                const long long pos = span.at(i + r);
-                const int off = offset(pos);
-                const T* from = dout + pos * p.cols + tile0 - off;
+                const uint32_t pos = span.at(i + r);
                 Vec16<T>* to = ring + (group * kEmbRows + r) * SLOT;
-                for (int k = lane; k * L < off + width; k += 32) {
-                    const T* src = from + k * L;
-                    if (VEC || (src >= dout && src + L <= dout + p.n * p.cols)) {
-                        copy16_async(to + k, src);
-                    } else {   // the packets at the tensor's ends: only what is inside
-                        Vec16<T> v;
+                if constexpr (VEC) {
+                    if (in) copy16_async(to + lane, mine + (long long)pos * p.cols);
+                } else {
+                    const int off = offset(pos);
+                    const T* from = dout + pos * p.cols + tile0 - off;
+                    for (int k = lane; k * L < off + width; k += 32) {
+                        const T* src = from + k * L;
+                        if (src >= dout && src + L <= dout + p.n * p.cols) {
+                            copy16_async(to + k, src);
+                        } else {   // the packets at the tensor's ends: only what is inside
+                            Vec16<T> v;
 #pragma unroll
-                        for (int l = 0; l < L; ++l) v.v[l] = src + l >= dout && src + l < dout + p.n * p.cols ? src[l] : Elem<T>::from_f32(0.0f);
-                        to[k] = v;
+                            for (int l = 0; l < L; ++l) v.v[l] = src + l >= dout && src + l < dout + p.n * p.cols ? src[l] : Elem<T>::from_f32(0.0f);
+                            to[k] = v;
+                        }
                     }
                 }
             }
@@ -663,36 +680,45 @@ __global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant_
     acc.clear();
     uint32_t cur = span.id(span.begin);
     bool head_part = span.head_part;
+    const unsigned long long change = span.change & ~(1ull << span.begin);   // the first pair of all begins nothing new
+    auto add = [&](int i, const Vec16<T>* slot) {   // pair i, whose piece is in `slot`
+        if (change >> i & 1) {
+            if (head_part) acc.write_part(p, chunk, 0, c0);
+            else acc.write(p, cur, c0);
+            head_part = false;
+            cur = span.id(i);
+            acc.clear();
+        }
+        const T* row = reinterpret_cast<const T*>(slot) + (VEC ? 0 : offset(span.at(i))) + lane * E;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if constexpr (E == 1) {
+                acc.v[q][0] += Elem<T>::to_f32(row[q * 32]);   // (behind the row's end: what is there, added to a column that is not written)
+            } else {
+                Vec16<T> v;
+                if constexpr (NP == 1) v = *reinterpret_cast<const Vec16<T>*>(row);
+                else *reinterpret_cast<int2*>(&v) = *reinterpret_cast<const int2*>(row + q * 32 * E);   // half a packet
+                float t[L];
+                unpack16<T>(v, t);
+#pragma unroll
+                for (int l = 0; l < E; l += 2) {
+                    const float2 a = __fadd2_rn(make_float2(acc.v[q][l], acc.v[q][l + 1]), make_float2(t[l], t[l + 1]));
+                    acc.v[q][l] = a.x;
+                    acc.v[q][l + 1] = a.y;
+                }
+            }
+        }
+    };
     int group = 0;
     for (int i0 = span.begin; i0 < span.end; i0 += kEmbRows) {
         copy_wait<kEmbGroups - 1>();
         __syncwarp();
+        const Vec16<T>* slot = ring + group * (kEmbRows * SLOT);
+        if (i0 + kEmbRows <= span.end) {
 #pragma unroll
-        for (int r = 0; r < kEmbRows; ++r) {
-            if (i0 + r >= span.end) break;
-            const uint32_t id = span.id(i0 + r);
-            if (id != cur) {
-                if (head_part) acc.write_part(p, chunk, 0, c0);
-                else acc.write(p, cur, c0);
-                head_part = false;
-                cur = id;
-                acc.clear();
-            }
-            const T* row = reinterpret_cast<const T*>(ring + (group * kEmbRows + r) * SLOT) + (VEC ? 0 : offset(span.at(i0 + r))) + lane * E;
-#pragma unroll
-            for (int q = 0; q < NP; ++q) {
-                if constexpr (E == 1) {
-                    acc.v[q][0] += Elem<T>::to_f32(row[q * 32]);   // (behind the row's end: what is there, added to a column that is not written)
-                } else {
-                    Vec16<T> v;
-                    if constexpr (NP == 1) v = *reinterpret_cast<const Vec16<T>*>(row);
-                    else *reinterpret_cast<int2*>(&v) = *reinterpret_cast<const int2*>(row + q * 32 * E);   // half a packet
-                    float t[L];
-                    unpack16<T>(v, t);
-#pragma unroll
-                    for (int l = 0; l < E; ++l) acc.v[q][l] += t[l];
-                }
-            }
+            for (int r = 0; r < kEmbRows; ++r) add(i0 + r, slot + r * SLOT);
+        } else {
+            for (int r = 0; i0 + r < span.end; ++r) add(i0 + r, slot + r * SLOT);
         }
         __syncwarp();
         fetch(group, i0 + kEmbGroups * kEmbRows);
