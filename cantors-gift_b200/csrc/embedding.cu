@@ -549,12 +549,15 @@ struct EmbLane {
     }
 };
 
+// Warps of a CTA of emb_grad_kernel. They share nothing, and a CTA ends with its longest: with eight of them 57344 rows of 1024 bf16 took 68 us
+// in all, with four 67, alone 65 (wide rows the other way: 16384 of 4096, 127, 127 and 131).
+constexpr int kEmbWarps = 1;
 constexpr int kZeroRows = 8;   // of a warp at a time
 // Table rows that no id names: a lane looks one row up in the sorted list, the warp zeroes those that are missing.
 template <typename G>
 __device__ __forceinline__ void emb_zero(const EmbGradParams& p, int lane, int warp) {
-    const long long step = (long long)p.zero_blocks * 8 * kZeroRows;
-    for (long long r0 = ((long long)blockIdx.x * 8 + warp) * kZeroRows; r0 < p.zero_rows; r0 += step) {
+    const long long step = (long long)p.zero_blocks * kEmbWarps * kZeroRows;
+    for (long long r0 = ((long long)blockIdx.x * kEmbWarps + warp) * kZeroRows; r0 < p.zero_rows; r0 += step) {
         bool missing = false;
         if (lane < kZeroRows && r0 + lane < p.zero_rows) {
             const uint32_t v = (uint32_t)(r0 + lane);
@@ -627,14 +630,14 @@ __device__ __forceinline__ EmbSpan emb_span(const EmbGradParams& p, long long ch
 // copied as the packets that cover it, one more than it fills, and a lane owns every 32nd column and finds it behind the row's own offset.
 constexpr int kEmbRows = 4, kEmbGroups = 4;   // rows of a copy group, groups in flight
 template <typename T, typename G, bool VEC>
-__global__ void __launch_bounds__(256, 3) emb_grad_kernel(const __grid_constant__ EmbGradParams p) {
+__global__ void __launch_bounds__(kEmbWarps * 32, 24 / kEmbWarps) emb_grad_kernel(const __grid_constant__ EmbGradParams p) {
     constexpr int L = Vec16<T>::N, E = !VEC ? 1 : Vec16<G>::N < L ? Vec16<G>::N : L, NP = L / E, SLOT = VEC ? 32 : 33;
     extern __shared__ float4 emb_smem4[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_trigger();
     pdl_wait();
     if (blockIdx.x < p.zero_blocks) return emb_zero<G>(p, lane, warp);
-    const long long unit = (long long)(blockIdx.x - p.zero_blocks) * 8 + warp;
+    const long long unit = (long long)(blockIdx.x - p.zero_blocks) * kEmbWarps + warp;
     const long long chunk = unit / p.tiles;
     if (chunk >= p.chunks) return;
     const long long tile0 = (unit - chunk * p.tiles) * (32 * L), c0 = tile0 + lane * E;
@@ -874,15 +877,15 @@ static int emb_backward(EmbGradParams p, cudaStream_t s) {
     constexpr int L = Vec16<T>::N;
     const bool vec = p.cols % L == 0 && aligned_to(p.dout, 16) && aligned_to(p.dtable, 16);
     p.tiles = (int)((p.cols + 32 * L - 1) / (32 * L));
-    const long long zero_cap = (long long)sm_count() * 32, want = (p.zero_rows + 8 * kZeroRows - 1) / (8 * kZeroRows);
+    const long long zero_cap = (long long)sm_count() * 256 / kEmbWarps, want = (p.zero_rows + kEmbWarps * kZeroRows - 1) / (kEmbWarps * kZeroRows);
     p.zero_blocks = (int)(want < zero_cap ? want : zero_cap);
-    const long long blocks = (p.chunks * p.tiles + 7) / 8 + p.zero_blocks;
+    const long long blocks = (p.chunks * p.tiles + kEmbWarps - 1) / kEmbWarps + p.zero_blocks;
     if (blocks > 0x7fffffffll) return CG_B200_ERR_UNSUPPORTED;
     auto k = vec ? emb_grad_kernel<T, G, true> : emb_grad_kernel<T, G, false>;
-    const int smem = 8 * kEmbGroups * kEmbRows * (vec ? 32 : 33) * 16;
+    const int smem = kEmbWarps * kEmbGroups * kEmbRows * (vec ? 32 : 33) * 16;
     if (blocks > 0) {
         CGB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        CGB_CUDA(launch_pdl(k, (unsigned)blocks, 256, smem, s, p));
+        CGB_CUDA(launch_pdl(k, (unsigned)blocks, kEmbWarps * 32, smem, s, p));
     }
     if (p.n > kChunk) {   // fewer cannot cover a chunk and reach beyond it
         const int e = p.cols % 4 == 0 ? 4 : 1;
