@@ -97,9 +97,10 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
 }
 
 // ---- asynchronous copies into shared memory -----------------------------------------------------------
-__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
+__device__ __forceinline__ void copy16_async(uint32_t shared_address, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address), "l"(global) : "memory");
 }
+__device__ __forceinline__ void copy16_async(void* smem, const void* global) { copy16_async((uint32_t)__cvta_generic_to_shared(smem), global); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // until at most N of this thread's groups are under way
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

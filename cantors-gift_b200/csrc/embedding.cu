@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __g
     if (me == 0 && threadIdx.x == 0) *p.joins = 0;
 }
 
-constexpr long long kZeroBase = 30, kZeroPerRound = 12;   // MB cleared beside a sort of so many rounds
+// MB cleared beside a sort of so many rounds: what the six or so other clusters that find room write in its time (a sort of four rounds with
+// 120 MB beside it took 37 us, with 78 MB 21, with none 21)
+constexpr long long kZeroBase = 30, kZeroPerRound = 12;
 
 template <typename I, int ROUNDS>
 static cudaError_t sort_cluster(const SortParams& p, int passes, int digit_bits, int ctas, cudaStream_t s) {

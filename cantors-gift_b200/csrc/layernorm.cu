@@ -6,11 +6,12 @@
 //   backward  dx = rstd * (g - sum(g) / C - h * sum(g * h) / C)         (the two sums over the row)
 //             dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy
 //
-// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once. One CTA per SM walks the rows; its threads
-// form groups, a row (forward: two rows at once) to a group: eight threads, a warp, or up to 16 warps with a barrier of their own. A row is
-// 16-byte packets, packet j * TPR + t for thread t, copied asynchronously into shared memory up to three rows ahead: a thread copies and
-// reads its own packets only, so nothing but its own copies has to be waited for, and loads stay in flight while rows are reduced
-// without costing registers. In the backward pass each thread adds its columns' share of dgamma and dbeta to fp32 registers over all
+// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once (measured: 65536 x 1024 bf16 forward 46 - 50 us, 82 - 88 % of the
+// copy rate; 32768 x 4096 bf16 backward 130 - 144 us, 85 - 94 %; the spread is the SM clock's, since what remains is latency). One CTA per SM
+// walks the rows; its threads form groups, a row (forward: two rows at once) to a group: eight threads, a warp, or up to 16 warps with a
+// barrier of their own. A row is 16-byte packets, packet j * TPR + t for thread t, copied asynchronously into shared memory up to three
+// rows ahead: a thread copies and reads its own packets only, so nothing but its own copies has to be waited for, and loads stay in flight
+// while rows are reduced without costing registers (loads into registers, with a row's lookahead: 59 and 229 us). In the backward pass each thread adds its columns' share of dgamma and dbeta to fp32 registers over all
 // rows of its group; the groups' sums are joined in shared memory, the CTAs' sums go to the workspace and a second kernel adds them up,
 // all in a fixed order, so the result does not depend on timing. Arithmetic is on fp32 pairs: with single instructions the backward
 // pass is bound by issue before it is bound by HBM.
@@ -90,9 +91,9 @@ __device__ __forceinline__ void row_sum(LnSums<N>& s, LnSums<N>* scratch, int& p
 
 // The same for two values, which is what the kernels below reduce, with half the shuffles: from the first exchange on, one half of the lanes
 // adds up the first value and the other half the second. Behind the barrier every thread reads all warps' sums, two to a 16-byte read;
-// entries from `warps` on are zero (row_sum2_prepare).
+// entries from `warps` on are zero (row_sum2_prepare). warp: the thread's in its group.
 template <bool SUB>
-__device__ __forceinline__ void row_sum2(LnSums<2>& s, LnSums<2>* scratch, int& phase, int bar, int warps) {
+__device__ __forceinline__ void row_sum2(LnSums<2>& s, LnSums<2>* scratch, int& phase, int bar, int warps, int warp) {
     constexpr int HALF = SUB ? 4 : 16;
     const int lane = threadIdx.x & 31;
     const unsigned mask = SUB ? 0xffu << (lane & 24) : 0xffffffffu;
@@ -108,7 +109,7 @@ __device__ __forceinline__ void row_sum2(LnSums<2>& s, LnSums<2>* scratch, int& 
     }
     LnSums<2>* at = scratch + phase;
     phase ^= 16;
-    if ((lane & 15) == 0) at[(threadIdx.x >> 5) % warps].v[lane >> 4] = v;
+    if ((lane & 15) == 0) at[warp].v[lane >> 4] = v;
     asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
     const float4* q = reinterpret_cast<const float4*>(at);
     auto two = [&](int i) {
@@ -220,13 +221,15 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
     auto live = [&](int j) { return j * tpr + lane < span.packets; };
     const T* src = static_cast<const T*>(p.in) + first * p.cols + c_lane;   // of the next row to fetch
     int to_fetch = left;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     auto fetch = [&](Vec16<T>* slot) {
+        const uint32_t to = ring_at + (uint32_t)(slot - ring) * 16;
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (to_fetch-- > 0) {
 #pragma unroll
                 for (int j = 0; j < CH; ++j)
-                    if (live(j)) copy16_async(slot + (r * CH + j) * kLnThreads, src + j * c_step);
+                    if (live(j)) copy16_async(to + (r * CH + j) * (kLnThreads * 16), src + j * c_step);
                 src += step * p.cols;
             } else if (r > 0) {
 #pragma unroll
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
             if constexpr (RAGGED) t = __fadd2_rn(t, make_float2(e[r][0], e[r][1]));
             s.v[r] = t.x + t.y;
         }
-        if constexpr (R == 2) row_sum2<SUB>(s, scratch, phase, group + 1, warps);
+        if constexpr (R == 2) row_sum2<SUB>(s, scratch, phase, group + 1, warps, lane >> 5);
         else row_sum<SUB>(s, scratch, phase, group + 1, warps);
         float mean[R];
 #pragma unroll
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
             }
             s.v[r] = t.x + t.y;
         }
-        if constexpr (R == 2) row_sum2<SUB>(s, scratch, phase, group + 1, warps);
+        if constexpr (R == 2) row_sum2<SUB>(s, scratch, phase, group + 1, warps, lane >> 5);
         else row_sum<SUB>(s, scratch, phase, group + 1, warps);
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -383,15 +386,17 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
     const T* x_src = static_cast<const T*>(p.in) + first * p.cols + c_lane;
     const T* y_src = static_cast<const T*>(p.dout) + first * p.cols + c_lane;
     int to_fetch = left;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     auto fetch = [&](Vec16<T>* slot) {
+        const uint32_t to = ring_at + (uint32_t)(slot - ring) * 16;
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (to_fetch-- > 0) {
 #pragma unroll
                 for (int j = 0; j < CH; ++j)
                     if (live(j)) {
-                        copy16_async(slot + (r * 2 * CH + j) * kLnThreads, x_src + j * c_step);
-                        copy16_async(slot + (r * 2 * CH + CH + j) * kLnThreads, y_src + j * c_step);
+                        copy16_async(to + (r * 2 * CH + j) * (kLnThreads * 16), x_src + j * c_step);
+                        copy16_async(to + (r * 2 * CH + CH + j) * (kLnThreads * 16), y_src + j * c_step);
                     }
                 x_src += step * p.cols;
                 y_src += step * p.cols;
@@ -407,14 +412,17 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
             if (!live(j)) ring[(i * CH + j) * kLnThreads] = Vec16<T>{};
     for (int i = 0; i < sh.stages; ++i) fetch(ring + i * R * 2 * CH * kLnThreads);
     float mean_n[R], rstd_n[R];   // of the next rows, read in time; zero for rows that are not there
+    const float *mean_at = p.mean + first, *rstd_at = p.rstd + first;
     auto statistics = [&](int i) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             mean_n[r] = rstd_n[r] = 0.0f;
             if (i + r < left) {
-                mean_n[r] = p.mean[first + (i + r) * step];
-                rstd_n[r] = p.rstd[first + (i + r) * step];
+                mean_n[r] = *mean_at;
+                rstd_n[r] = *rstd_at;
             }
+            mean_at += step;
+            rstd_at += step;
         }
     };
     statistics(0);
@@ -526,7 +534,7 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_bwd_kernel(const __grid_cons
             s.v[2 * r] = s1.x + s1.y;
             s.v[2 * r + 1] = s2.x + s2.y;
         }
-        if constexpr (R == 1) row_sum2<SUB>(s, scratch, phase, group + 1, warps);
+        if constexpr (R == 1) row_sum2<SUB>(s, scratch, phase, group + 1, warps, lane >> 5);
         else row_sum<SUB>(s, scratch, phase, group + 1, warps);
 #pragma unroll
         for (int r = 0; r < R; ++r)
