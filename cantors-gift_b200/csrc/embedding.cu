@@ -734,10 +734,10 @@ __global__ void __launch_bounds__(kEmbWarps * 32, 24 / kEmbWarps) emb_grad_kerne
     else acc.write(p, cur, c0);
 }
 
-// Joins the sums of an id over the chunks that it covers: a CTA per id and 32 * E columns, sixteen strands of sums, each in order.
+// Joins the sums of an id over the chunks that it covers: a CTA per id and 32 * E columns, eight strands of sums, each in order.
 template <typename G, int E>
-__global__ void __launch_bounds__(512) emb_join_kernel(const __grid_constant__ EmbGradParams p) {
-    __shared__ float sum[16][32 * E + 1];
+__global__ void __launch_bounds__(256) emb_join_kernel(const __grid_constant__ EmbGradParams p) {
+    __shared__ float sum[8][32 * E + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_trigger();
     pdl_wait();
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(512) emb_join_kernel(const __grid_constant__ E
         if (c < p.cols) {
             if (warp == 0) add(p.part + (chunk * 2 + 1) * p.cols + c);
 #pragma unroll 8
-            for (long long k = chunk + 1 + warp; k <= last; k += 16) add(p.part + k * 2 * p.cols + c);
+            for (long long k = chunk + 1 + warp; k <= last; k += 8) add(p.part + k * 2 * p.cols + c);
         }
         __syncthreads();
 #pragma unroll
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(512) emb_join_kernel(const __grid_constant__ E
         if (threadIdx.x < 32 * E && cc < p.cols) {
             float f = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 16; ++w) f += sum[w][threadIdx.x];
+            for (int w = 0; w < 8; ++w) f += sum[w][threadIdx.x];
             G* dst = static_cast<G*>(p.dtable) + (long long)id * p.cols + cc;
             f *= p.scale;
             if (p.accumulate) f += Elem<G>::to_f32(*dst);
@@ -891,8 +891,8 @@ static int emb_backward(EmbGradParams p, cudaStream_t s) {
     }
     if (p.n > kChunk) {   // fewer cannot cover a chunk and reach beyond it
         const int e = p.cols % 4 == 0 ? 4 : 1;
-        const long long units = p.chunks * ((p.cols + 32 * e - 1) / (32 * e)), cap = (long long)sm_count() * 4;
-        CGB_CUDA(launch_pdl(e == 4 ? emb_join_kernel<G, 4> : emb_join_kernel<G, 1>, (unsigned)(units < cap ? units : cap), 512, 0, s, p));
+        const long long units = p.chunks * ((p.cols + 32 * e - 1) / (32 * e)), cap = (long long)sm_count() * 8;
+        CGB_CUDA(launch_pdl(e == 4 ? emb_join_kernel<G, 4> : emb_join_kernel<G, 1>, (unsigned)(units < cap ? units : cap), 256, 0, s, p));
     }
     return CG_B200_OK;
 }
