@@ -100,6 +100,15 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
 __device__ __forceinline__ void copy16_async(uint32_t shared_address, const void* global) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address), "l"(global) : "memory");
 }
+// the same with a policy for L2, such as that of data read once by a kernel: it leaves first when L2 needs room
+__device__ __forceinline__ uint64_t leaves_l2_first() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void copy16_async(uint32_t shared_address, const void* global, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(shared_address), "l"(global), "l"(policy) : "memory");
+}
 __device__ __forceinline__ void copy16_async(void* smem, const void* global) { copy16_async((uint32_t)__cvta_generic_to_shared(smem), global); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // until at most N of this thread's groups are under way

@@ -6,14 +6,15 @@
 //   backward  dx = rstd * (g - sum(g) / C - h * sum(g * h) / C)         (the two sums over the row)
 //             dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy
 //
-// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once (measured: 65536 x 1024 bf16 forward 46 - 50 us, 82 - 88 % of the
-// copy rate; 32768 x 4096 bf16 backward 130 - 144 us, 85 - 94 %; the spread is the SM clock's, since what remains is latency). One CTA per SM
+// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once (measured: 65536 x 1024 bf16 forward 49 us, 84 % of the copy
+// rate; 32768 x 4096 bf16 backward 129 - 134 us, 92 - 95 %; 14000 x 8000 fp32 148 and 212 us, 92 and 97 %). One CTA per SM
 // walks the rows; its threads form groups, a row (forward: two rows at once) to a group: eight threads, a warp, or up to 16 warps with a
-// barrier of their own. A row is 16-byte packets, packet j * TPR + t for thread t, copied asynchronously into shared memory up to three
-// rows ahead: a thread copies and reads its own packets only, so nothing but its own copies has to be waited for, and loads stay in flight
-// while rows are reduced without costing registers (loads into registers, with a row's lookahead: 59 and 229 us). In the backward pass each thread adds its columns' share of dgamma and dbeta to fp32 registers over all
-// rows of its group; the groups' sums are joined in shared memory, the CTAs' sums go to the workspace and a second kernel adds them up,
-// all in a fixed order, so the result does not depend on timing. Arithmetic is on fp32 pairs: with single instructions the backward
+// barrier of their own. A row is 16-byte packets, packet j * TPR + t for thread t, copied asynchronously into shared memory ahead of
+// its use: a thread copies and reads its own packets only, so nothing but its own copies has to be waited for, and loads stay in flight
+// while rows are reduced without costing registers (loads into registers, with a row's lookahead: 59 and 229 us). In the backward pass
+// each thread adds its columns' share of dgamma and dbeta to fp32 registers over all rows of its group; the groups' sums are joined in
+// shared memory, the CTAs' sums go to the workspace and a second kernel adds them up, all in a fixed order, so the result does not
+// depend on timing. Arithmetic is on fp32 pairs: with single instructions the backward
 // pass is bound by issue before it is bound by HBM.
 //
 // Rows whose width no packet divides start at a different offset from a 16-byte boundary each. The rows of one CTA are gridDim.x apart, a
@@ -198,7 +199,7 @@ __device__ __forceinline__ LnSingles ln_singles(const LnSpan& s, int lane) {
 struct LnShape {
     int tpr;        // threads per row: 8 when SUB, else a multiple of 32
     int groups;     // rows at a time
-    int stages;     // rows ahead
+    int stages;     // steps of a group in shared memory: the one in work and the next ones
 };
 
 // CH packets per thread; the parameters stay in registers. A group takes R rows at a time: the dependent reductions of a row are latency,
@@ -222,6 +223,9 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
     const T* src = static_cast<const T*>(p.in) + first * p.cols + c_lane;   // of the next row to fetch
     int to_fetch = left;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    // Rows read first make room in L2 for rows being written: 131072 x 512 bf16 51.3 -> 49.4 us, 24576 x 4096 fp32 145 -> 139 us (bf16 of
+    // that shape 66 -> 69 us). Not of ragged rows, whose ends share sectors with their neighbours: 32700 x 1027 fp32 51.1 -> 53.6 us.
+    const uint64_t once = leaves_l2_first();
     auto fetch = [&](Vec16<T>* slot) {
         const uint32_t to = ring_at + (uint32_t)(slot - ring) * 16;
 #pragma unroll
@@ -229,7 +233,10 @@ __global__ void __launch_bounds__(kLnThreads, 1) ln_fwd_kernel(const __grid_cons
             if (to_fetch-- > 0) {
 #pragma unroll
                 for (int j = 0; j < CH; ++j)
-                    if (live(j)) copy16_async(to + (r * CH + j) * (kLnThreads * 16), src + j * c_step);
+                    if (live(j)) {
+                        if constexpr (RAGGED) copy16_async(to + (r * CH + j) * (kLnThreads * 16), src + j * c_step);
+                        else copy16_async(to + (r * CH + j) * (kLnThreads * 16), src + j * c_step, once);
+                    }
                 src += step * p.cols;
             } else if (r > 0) {
 #pragma unroll
@@ -732,7 +739,13 @@ static int ln_launch(const LnParams& p, bool ragged, int* parts, cudaStream_t s)
     if (SUB) sh.groups = (sh.groups + 3) / 4 * 4;   // whole warps
     const int threads = sh.groups * sh.tpr;
     const size_t row = (size_t)R * CH * kLnThreads * 16 * (BWD ? 2 : 1);
-    sh.stages = 3;
+    // Steps in shared memory, the one in work included. More rows at once upset the memory's order of service, fewer leave it idle while
+    // rows are reduced. The short rows of SUB take three (524288 x 64 bf16 forward 27.4 us, with two 30.6). 16-bit rows, which compute twice
+    // as much per byte, take two (65536 x 1024 bf16 forward 49.5 us, with three 51.7; 24576 x 4096 69 us, with one 74). fp32 rows take
+    // one where enough threads have rows (24576 x 4096 forward 133 us and backward 192, with two 137 and 203; 16000 x 2500 backward 82 and 93),
+    // two where one group leaves many threads out (6000 x 5000, 320 threads: forward 43 us and backward 63, with one 48 and 72).
+    const bool one = sizeof(T) == 4 && (sh.groups > 1 || threads >= (BWD ? 448 : 352));
+    sh.stages = SUB ? 3 : one ? 1 : 2;
     while (row * sh.stages > 208 * 1024) --sh.stages;   // of 227 KB, with the static scratch and what the system keeps per CTA
     size_t smem = row * sh.stages;
     const size_t join = (size_t)(threads * CH * L + sh.groups * 16) * 4;
