@@ -8,8 +8,8 @@
 // (113M gradients, bf16 into fp32: 907 MB in 159 us, 87 % of the copy rate).
 // The tensors' addresses, lengths and types travel by value in the kernel's parameters, so nothing is copied to the device first and
 // nothing is kept between calls. The list is cut into as many equal pieces as there are CTAs; squares are added in fp32 per 16-byte packet
-// and in fp64 beyond it, and every CTA leaves one fp64 sum in the workspace. The scaling kernel's CTAs each add those sums up in the same fixed order, so the norm does not depend on timing, and walk
-// their pieces backwards: what the norm pass read last is still in L2.
+// and in fp64 beyond it, and every CTA leaves one fp64 sum in the workspace. The scaling kernel's CTAs each add those sums up in the same
+// fixed order, so the norm does not depend on timing, and walk their pieces backwards: what the norm pass read last is still in L2.
 #include <float.h>
 #include <stdlib.h>
 
@@ -217,17 +217,18 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_only_kernel(const doub
 
 static long long clip_grid_cap() { return (long long)sm_count() * kClipCtas; }
 
-// Nothing may be written twice, and nothing written may be another's input: a tensor is scaled in place, or into memory of its own. The
-// address ranges are sorted and swept once.
+// Nothing may be written twice, and nothing written may be another's input: a tensor is scaled in place, or into memory of its own, and
+// the norm, written while the list is still read, is apart from all. The address ranges are sorted and swept once.
 struct ClipRange {
     uintptr_t from, to;
     bool written;
 };
-static int clip_check_overlap(const cg_b200_grad* g, int64_t count) {
-    ClipRange few[2 * kClipShort];
+static int clip_check_overlap(const cg_b200_grad* g, int64_t count, const float* norm) {
+    ClipRange few[2 * kClipShort + 1];
     ClipRange* r = few;
-    if (count > kClipShort && !(r = static_cast<ClipRange*>(malloc((size_t)count * 2 * sizeof(ClipRange))))) return CG_B200_ERR_INVALID_ARG;
+    if (count > kClipShort && !(r = static_cast<ClipRange*>(malloc(((size_t)count * 2 + 1) * sizeof(ClipRange))))) return CG_B200_ERR_INVALID_ARG;
     int64_t n = 0;
+    if (norm) r[n++] = {reinterpret_cast<uintptr_t>(norm), reinterpret_cast<uintptr_t>(norm) + sizeof(float), true};
     for (int64_t i = 0; i < count; ++i) {
         if (g[i].n == 0) continue;
         const uintptr_t in = reinterpret_cast<uintptr_t>(g[i].in), out = reinterpret_cast<uintptr_t>(g[i].out);
@@ -246,7 +247,7 @@ static int clip_check_overlap(const cg_b200_grad* g, int64_t count) {
     return bad ? CG_B200_ERR_INVALID_ARG : CG_B200_OK;
 }
 
-static int clip_check(const cg_b200_grad* g, int64_t count, bool scale) {
+static int clip_check(const cg_b200_grad* g, int64_t count, const float* norm, bool scale) {
     if (count < 0 || count > (1 << 20)) return CG_B200_ERR_INVALID_ARG;
     if (count > 0 && !g) return CG_B200_ERR_NULL_POINTER;
     for (int64_t i = 0; i < count; ++i) {
@@ -258,7 +259,7 @@ static int clip_check(const cg_b200_grad* g, int64_t count, bool scale) {
         if (!scale) continue;
         if (!aligned_to(g[i].out, dtype_bytes(g[i].out_dtype))) return CG_B200_ERR_MISALIGNED;
     }
-    return scale ? clip_check_overlap(g, count) : CG_B200_OK;
+    return scale ? clip_check_overlap(g, count, norm) : CG_B200_OK;
 }
 
 static size_t clip_workspace(int64_t count) {
@@ -320,7 +321,7 @@ static int clip_run(const cg_b200_grad* g, int64_t count, float max_norm, float*
 
 static int clip_entry(const cg_b200_grad* grads, int64_t count, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
                       bool scale, void* stream) {
-    int st = clip_check(grads, count, scale);
+    int st = clip_check(grads, count, norm, scale);
     if (st) return st;
     if (!norm) return CG_B200_ERR_NULL_POINTER;
     if (!aligned_to(norm, 4) || !aligned_to(workspace, 16)) return CG_B200_ERR_MISALIGNED;

@@ -336,7 +336,7 @@ def grad_norm(grads, norm=None, stream=None):
 def clip_grad_norm(grads, max_norm, out=None, norm=None, stream=None):
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)) and returns their norm before it (0-dim fp32, on the device;
     nothing waits for the GPU). In place, or into `out`: one tensor for each, of as many elements, of its gradient's dtype or
-    fp32, in memory of its own. No tensor may be in the list twice."""
+    fp32, in memory of its own, as is `norm` if it is given. No tensor may be in the list twice."""
     return _norm_call(list(grads), max_norm, out, norm, stream)
 
 

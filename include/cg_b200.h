@@ -256,10 +256,10 @@ int cg_b200_reduce(int dtype, int op, const void* in, void* out, int64_t outer, 
  *   clip: out = in * min(1, max_norm / (norm + 1e-6)), each rounded once to out_dtype
  * `host_grads` is read before the call returns. A tensor is `n` contiguous elements of any alignment down to its element
  * size; out_dtype is `dtype` or CG_B200_F32, out may be `in` itself when the types agree and otherwise must not overlap
- * any input. No tensor may be written twice. *norm is fp32 on the device. Squares are summed in fp64 beyond 16-byte
- * packets, in a fixed order; a list whose norm is infinite or not a number is scaled by the factor that the formula
- * gives (0 or NaN). cg_b200_grad_norm ignores out, out_dtype. count <= 2^20; count == 0 gives norm 0. The workspace must
- * be 16-byte aligned; two calls that can run at the same time need one each. */
+ * any input. No tensor may be written twice, and *norm (fp32 on the device) is part of none. Squares are summed in fp64
+ * beyond 16-byte packets, in a fixed order; a list whose norm is infinite or not a number is scaled by the factor that the
+ * formula gives (0 or NaN). cg_b200_grad_norm ignores out, out_dtype. count <= 2^20; count == 0 gives norm 0. The workspace
+ * must be 16-byte aligned; two calls that can run at the same time need one each. */
 typedef struct cg_b200_grad {
     const void* in;
     void*       out;

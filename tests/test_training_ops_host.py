@@ -130,6 +130,22 @@ def test_clip_refusals(cgb):
     assert L.cg_b200_grad_norm(t, 2, None, P, need.value, None) == capi.ERR_NULL_POINTER   # outputs are not looked at, norm is
 
 
+@pytest.mark.parametrize("count", [2, 100])   # with the address ranges on the stack, and allocated
+def test_clip_norm_apart_from_the_list(cgb, count):
+    """The norm is written while the list is still being read, so it may be no part of a gradient or of an output."""
+    capi, L = cgb.capi, cgb.lib()
+    t = (capi.Grad * count)()
+    for i, e in enumerate(t):
+        e.in_, e.out, e.n, e.dtype, e.out_dtype = (1 << 16) + i * 1024, (1 << 20) + i * 1024, 100, capi.F32, capi.F32
+    last = count - 1
+    # a call that gets past this check is refused for its missing workspace
+    for at, status in (((1 << 16) - 4, capi.ERR_WORKSPACE), (1 << 16, capi.ERR_INVALID_ARG),
+                       ((1 << 16) + last * 1024 + 396, capi.ERR_INVALID_ARG), ((1 << 16) + last * 1024 + 400, capi.ERR_WORKSPACE),
+                       ((1 << 20) - 4, capi.ERR_WORKSPACE), (1 << 20, capi.ERR_INVALID_ARG),
+                       ((1 << 20) + last * 1024 + 396, capi.ERR_INVALID_ARG), ((1 << 20) + last * 1024 + 400, capi.ERR_WORKSPACE)):
+        assert L.cg_b200_clip_grad_norm(t, count, 1.0, C.c_void_p(at), None, 0, None) == status, hex(at)
+
+
 def test_python_entry_points_take_cuda_tensors(cgb):
     import torch
     from cantors_gift_b200 import ops
