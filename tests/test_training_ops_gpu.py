@@ -317,6 +317,20 @@ def test_embedding_gradient_accumulates(ops, types, n, vocab, cols):
     assert torch.equal(got[count == 0], old[count == 0])
 
 
+@pytest.mark.parametrize("n,vocab,cols", [(131072, 32000, 4), (131073, 3, 8), (600011, 32000, 5), (1048583, 3, 4), (1048583, 1 << 20, 4)])
+def test_embedding_gradient_of_many_ids(ops, n, vocab, cols):
+    """Sorts of one to three passes with hundreds of tiles. Integers whose sums stay below 2^24: exact in any order of additions."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    dy = torch.randint(-4, 5, (n, cols), device="cuda", generator=g).float()
+    ids = (torch.rand(n, device="cuda", generator=g) ** 2 * (vocab + 1)).long() - 1
+    inside = ids >= 0
+    want = torch.zeros(vocab, cols, device="cuda", dtype=torch.float64).index_add_(0, ids[inside], dy[inside].double())
+    obuf, out = guarded((vocab, cols), torch.float32)
+    got = ops.embedding_backward(dy, ids, vocab, out=out)
+    assert torch.equal(got.double(), want)
+    assert_guards(obuf, out, "gradient")
+
+
 def test_embedding_gradient_of_one_id_everywhere(ops):
     """Every pair names one row: the sums of all chunks are joined (1250 of them)."""
     n, vocab, cols = 40000, 1000, 72
