@@ -45,6 +45,8 @@ struct LnParams {
 
 constexpr int kLnThreads = 512;   // of a CTA at most: 128 registers each
 constexpr int kLnWarps = kLnThreads / 32;
+// Dynamic shared memory of a CTA at most: of 227 KB, with the static scratch and what the system keeps per CTA
+constexpr int kLnSmem = 208 * 1024;
 
 // Sums of N values over the threads that share a row (8 lanes of a warp when SUB, else `warps` warps); every thread gets them. The warps
 // of a group meet at barrier `bar`; two scratch halves take turns, so one barrier per call is enough.
@@ -746,20 +748,23 @@ static int ln_launch(const LnParams& p, bool ragged, int* parts, cudaStream_t s)
     // two where one group leaves many threads out (6000 x 5000, 320 threads: forward 43 us and backward 63, with one 48 and 72).
     const bool one = sizeof(T) == 4 && (sh.groups > 1 || threads >= (BWD ? 448 : 352));
     sh.stages = SUB ? 3 : one ? 1 : 2;
-    while (row * sh.stages > 208 * 1024) --sh.stages;   // of 227 KB, with the static scratch and what the system keeps per CTA
+    while (row * sh.stages > kLnSmem) --sh.stages;
     size_t smem = row * sh.stages;
     const size_t join = (size_t)(threads * CH * L + sh.groups * 16) * 4;
+    static_assert((kLnThreads * CH * L + kLnThreads / 8 * 16) * 4 <= kLnSmem, "the join fits for every shape");
     if (BWD && smem < join) smem = join;
     long long grid = (p.rows + sh.groups - 1) / sh.groups;
     if (grid > sms) grid = sms;
     if (ragged) grid = grid >= L ? grid / L * L : L;   // down: a CTA more than fits would be a wave of its own
     if (parts) *parts = (int)grid;
+    // The limit is the kernel's, not the launch's, and other host threads launch the same kernel with other shapes: every call sets the same
+    // one. (Set to each call's own size, it was lowered between another thread's setting and its launch, which was then refused.)
 #define CGB_LN_GO(M)                                                                                                        \
     {                                                                                                                       \
         void (*k)(const LnParams, const LnShape);                                                                           \
         if constexpr (BWD) k = ln_bwd_kernel<T, TP, CH, R, SUB, M>;                                                         \
         else k = ln_fwd_kernel<T, TP, CH, R, SUB, M>;                                                                       \
-        if (smem > 32 * 1024) CGB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));    \
+        if (smem > 32 * 1024) CGB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kLnSmem));      \
         k<<<(unsigned)grid, threads, smem, s>>>(p, sh);                                                                     \
     }
     if (ragged) CGB_LN_GO(true) else CGB_LN_GO(false)
