@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_training_ops_gpu import normal
+from test_training_ops_gpu import CHAIN, DTYPES, assert_within, check_ln_backward, check_ln_forward, guarded, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,61 @@ def test_layernorm_graph_of_two_sizes_replays(ops):
     for got, want in zip(gots, wants):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+# ---- long sums ----------------------------------------------------------------------------------------------
+def steady_rows(rows, cols, dtype, shift):
+    """x and dy with the same values in every row: the sums over rows are rows times one term, and the rounding errors of a running sum,
+    all of one sign between two powers of two, add up instead of cancelling. Mean 0 and rstd 1 are given, so that h is x."""
+    # 16-bit values, so that x * dy is exact in fp32
+    u, v = normal(cols, seed=1, dtype=torch.bfloat16), normal(cols, seed=2, dtype=torch.bfloat16)
+    _, x = guarded((rows, cols), dtype, 0)
+    _, dy = guarded((rows, cols), dtype, shift)
+    x.copy_(u)
+    dy.copy_(v)
+    return x, dy, u.double(), v.double()
+
+
+def check_weight_gradients(ops, rows, cols, dtype, shift, chain):
+    x, dy, u, v = steady_rows(rows, cols, dtype, shift)
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    gamma = torch.ones(cols, device="cuda")
+    _, dgamma, dbeta = ops.layernorm_backward(dy, x, mean, rstd, gamma, dx=x)
+    assert_within(dgamma, rows * u * v, rows * (u * v).abs(), "dgamma", chain=chain)
+    assert_within(dbeta, rows * v, rows * v.abs(), "dbeta", chain=chain)
+
+
+@pytest.mark.parametrize("rows,cols,shift", [(400000, 1024, 1), (40000, 16400, 0), (60000, 40000, 0)])
+def test_layernorm_streaming_weight_gradients_of_many_rows(ops, rows, cols, shift):
+    """Bases off by different amounts, and rows above 16384 columns: a thread adds 64 terms in fp32 and such sums in fp64, then eight
+    threads' sums and those of at most 152 slices in 16 strands follow: below CHAIN's 128 steps."""
+    check_weight_gradients(ops, rows, cols, torch.bfloat16, shift, CHAIN)
+
+
+@pytest.mark.parametrize("rows,cols", [(200000, 512), (30000, 16384)])
+def test_layernorm_weight_gradients_of_many_rows(ops, rows, cols):
+    """The register kernels: a group's threads add the rows of their group one after another. 512 columns of 16 bits have 16 groups to each of
+    148 CTAs, 16384 columns one group; 64 steps are left for the joins of 16 groups and of 148 CTAs in 16 strands."""
+    groups = 16 if cols == 512 else 1
+    chain = (-(-rows // (148 * groups)) + 64) * 2.0 ** -24
+    check_weight_gradients(ops, rows, cols, torch.bfloat16, 0, chain)
+
+
+def test_layernorm_weight_gradients_of_many_random_rows(ops):
+    rows, cols = 200000, 512
+    x, dy = normal(rows, cols, seed=3, dtype=torch.bfloat16), normal(rows, cols, seed=4, dtype=torch.bfloat16)
+    gamma, beta = normal(cols, seed=5, offset=1.0), normal(cols, seed=6)
+    _, mean, rstd = check_ln_forward(ops, x, gamma, beta)
+    check_ln_backward(ops, dy, x, mean, rstd, gamma)
+
+
+@pytest.mark.parametrize("dtype", ["F32", "BF16"])
+def test_layernorm_of_a_million_columns(ops, dtype):
+    """Two values in turn, so that a thread's running sum adds one and the same value every time."""
+    dt, cols = DTYPES[dtype], 1 << 20
+    x = torch.empty(2, cols, device="cuda", dtype=dt)
+    x[:, ::2], x[:, 1::2] = 0.1, 0.9
+    dy = torch.empty_like(x)
+    dy[:, ::2], dy[:, 1::2] = 0.7, 0.3
+    _, mean, rstd = check_ln_forward(ops, x, None, None)
+    check_ln_backward(ops, dy, x, mean, rstd, None)
