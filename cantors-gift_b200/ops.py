@@ -177,7 +177,7 @@ def _check_like(t, shape, dtype, what):
 
 def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, rstd=None, stream=None):
     """layernorm over the last axis that keeps its statistics: (y, mean, rstd), mean and rstd fp32 of shape x.shape[:-1].
-    gamma, beta: [cols] of x's dtype or fp32, each may be None. `out` may be x."""
+    gamma, beta: [cols] of x's dtype or fp32, each may be None. `out` may be x. Rows without columns have NaN statistics, 0 / 0."""
     _require_one_device(x, gamma, beta, out, mean, rstd)
     ctx = _elsewhere(x, stream)
     if ctx is not None:
@@ -200,6 +200,9 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, r
         _check_like(rstd, lead, torch.float32, "rstd")
     check(lib().cg_b200_layernorm_forward(dt, pt, x.data_ptr(), _addr(gamma), _addr(beta), eps, out.data_ptr(), mean.data_ptr(),
                                           rstd.data_ptr(), rows, cols, _raw_stream(x.get_device())), "layernorm_forward")
+    if cols == 0:   # the C entry does nothing then; bytes of 0xff are a NaN
+        for t in (mean, rstd):
+            check(lib().cg_b200_memset(t.data_ptr(), 0xff, 4 * rows, _raw_stream(x.get_device())), "memset")
     return out, mean, rstd
 
 

@@ -209,7 +209,8 @@ int cg_b200_softmax_layernorm(int dtype, const void* in, const void* gamma,
  * `param_dtype`, which is `dtype` or CG_B200_F32; mean, rstd are [rows] fp32. Any alignment down to the element size is
  * taken; 16-byte packets are used when the [rows, cols] tensors start at the same offset from a 16-byte boundary. Math
  * and sums are fp32, one rounding per result; the same inputs give the same bits on every call.
- * Forward: gamma, beta, mean, rstd may be NULL; in == out is allowed. Backward: gamma may be NULL (taken as 1); din,
+ * Forward: gamma, beta, mean, rstd may be NULL; in == out is allowed. cols == 0: both do nothing, so mean and rstd stay
+ * as they are. Backward: gamma may be NULL (taken as 1); din,
  * dgamma, dbeta may each be NULL, not all three; din may be `dout` or `in` itself, not overlap them otherwise. rows == 0:
  * dgamma and dbeta become zero. The workspace (16-byte aligned, contents undefined before and after) is used only
  * when dgamma or dbeta is asked for; two calls that can run at the same time need one each. */

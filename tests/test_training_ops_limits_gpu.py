@@ -134,3 +134,17 @@ def test_layernorm_of_a_million_columns(ops, dtype):
     dy[:, ::2], dy[:, 1::2] = 0.7, 0.3
     _, mean, rstd = check_ln_forward(ops, x, None, None)
     check_ln_backward(ops, dy, x, mean, rstd, None)
+
+
+# ---- tensors without columns ----------------------------------------------------------------------------------
+def test_layernorm_without_columns_gives_no_number(ops):
+    """The mean of nothing is 0 / 0: the statistics of such rows are NaN, in new tensors and in given ones."""
+    x = torch.empty(5, 0, device="cuda")
+    mean, rstd = torch.full((5,), 3.0, device="cuda"), torch.full((5,), 4.0, device="cuda")
+    y, m, r = ops.layernorm_forward(x, mean=mean, rstd=rstd)
+    assert m is mean and r is rstd and y.shape == (5, 0)
+    assert bool(torch.isnan(mean).all()) and bool(torch.isnan(rstd).all())
+    junk = torch.full((4096,), 7.0, device="cuda")   # what the allocator hands out next
+    del junk
+    _, m, r = ops.layernorm_forward(torch.empty(64, 64, 0, device="cuda"))
+    assert m.shape == r.shape == (64, 64) and bool(torch.isnan(m).all()) and bool(torch.isnan(r).all())
