@@ -34,6 +34,16 @@ inline bool dtype_ok(int dt) { return dt == CG_B200_F16 || dt == CG_B200_BF16 ||
 inline size_t dtype_bytes(int dt) { return dt == CG_B200_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// A tensor's bytes; none where the pointer is null. `count` elements of `size` bytes, as many as an address can count.
+struct Bytes {
+    uintptr_t at;
+    size_t n;
+    Bytes(const void* p, int64_t count, size_t size)
+        : at(reinterpret_cast<uintptr_t>(p)), n(!p ? 0 : (size_t)count > SIZE_MAX / size ? SIZE_MAX : (size_t)count * size) {}
+};
+inline bool overlap(const Bytes& a, const Bytes& b) { return a.n && b.n && (a.at < b.at ? b.at - a.at < a.n : a.at - b.at < b.n); }
+template <typename... B> bool overlaps_any(const Bytes& a, const B&... b) { return (overlap(a, b) || ...); }
+
 // Device error word shared by kernels with bounded waits (0 = no error).
 uint32_t* device_error_word();   // device pointer, lazily allocated per device; nullptr on failure
 

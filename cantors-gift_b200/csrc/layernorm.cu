@@ -916,6 +916,10 @@ extern "C" int cg_b200_layernorm_forward(int dtype, int param_dtype, const void*
     if (!aligned_to(in, esz) || !aligned_to(out, esz) || !aligned_to(gamma, psz) || !aligned_to(beta, psz) || !aligned_to(mean, 4) ||
         !aligned_to(rstd, 4))
         return CG_B200_ERR_MISALIGNED;
+    // what one CTA writes, another may still have to read
+    const Bytes x(in, rows * cols, esz), y(out, rows * cols, esz), g(gamma, cols, psz), b(beta, cols, psz), m(mean, rows, 4), r(rstd, rows, 4);
+    if ((in != out && overlap(y, x)) || overlaps_any(y, g, b, m, r) || overlaps_any(m, x, g, b, r) || overlaps_any(r, x, g, b))
+        return CG_B200_ERR_INVALID_ARG;
     int st = require_sm100();
     if (st) return st;
     LnParams p{};
@@ -955,6 +959,12 @@ extern "C" int cg_b200_layernorm_backward(int dtype, int param_dtype, const void
     size_t need = 0;
     cg_b200_layernorm_backward_workspace_bytes(rows, cols, &need);
     if ((dgamma || dbeta) && need > 0 && (!workspace || workspace_bytes < need)) return CG_B200_ERR_WORKSPACE;
+    // what one CTA writes, another may still have to read. (The weight gradients are written when all inputs have been read.)
+    const Bytes x(in, rows * cols, esz), dy(dout, rows * cols, esz), dx(din, rows * cols, esz), g(gamma, cols, psz), m(mean, rows, 4),
+        r(rstd, rows, 4), dg(dgamma, cols, psz), db(dbeta, cols, psz), ws(dgamma || dbeta ? workspace : nullptr, (int64_t)need, 1);
+    if ((din != in && overlap(dx, x)) || (din != dout && overlap(dx, dy)) || overlaps_any(dx, g, m, r, dg, db) || overlap(dg, db) ||
+        overlaps_any(ws, x, dy, dx, g, m, r, dg, db))
+        return CG_B200_ERR_INVALID_ARG;
     int st = require_sm100();
     if (st) return st;
     LnParams p{};

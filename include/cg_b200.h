@@ -209,11 +209,14 @@ int cg_b200_softmax_layernorm(int dtype, const void* in, const void* gamma,
  * `param_dtype`, which is `dtype` or CG_B200_F32; mean, rstd are [rows] fp32. Any alignment down to the element size is
  * taken; 16-byte packets are used when the [rows, cols] tensors start at the same offset from a 16-byte boundary. Math
  * and sums are fp32, one rounding per result; the same inputs give the same bits on every call.
- * Forward: gamma, beta, mean, rstd may be NULL; in == out is allowed. cols == 0: both do nothing, so mean and rstd stay
- * as they are. Backward: gamma may be NULL (taken as 1); din,
- * dgamma, dbeta may each be NULL, not all three; din may be `dout` or `in` itself, not overlap them otherwise. rows == 0:
- * dgamma and dbeta become zero. The workspace (16-byte aligned, contents undefined before and after) is used only
- * when dgamma or dbeta is asked for; two calls that can run at the same time need one each. */
+ * cols == 0: both do nothing, so mean and rstd stay as they are.
+ * Forward: gamma, beta, mean, rstd may be NULL. out may be `in` itself; apart from that out, mean and rstd overlap neither
+ * an input nor one another (CG_B200_ERR_INVALID_ARG).
+ * Backward: gamma may be NULL (taken as 1); din, dgamma, dbeta may each be NULL, not all three. din may be `dout` or `in`
+ * itself; apart from that din and the workspace overlap nothing else of the call, nor do dgamma and dbeta one another
+ * (CG_B200_ERR_INVALID_ARG). rows == 0: dgamma and dbeta become zero. The workspace (16-byte aligned, contents
+ * undefined before and after) is used only when dgamma or dbeta is asked for; two calls that can run at the same time
+ * need one each. */
 int cg_b200_layernorm_forward(int dtype, int param_dtype, const void* in, const void* gamma, const void* beta, float eps,
                               void* out, float* mean, float* rstd, int64_t rows, int64_t cols, void* stream);
 int cg_b200_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols, size_t* bytes);

@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_training_ops_gpu import CHAIN, DTYPES, assert_within, check_ln_backward, check_ln_forward, guarded, normal
+from test_training_ops_gpu import CHAIN, DTYPES, assert_within, check_ln_backward, check_ln_forward, guarded, ln_backward_reference, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,43 @@ def test_layernorm_without_columns_gives_no_number(ops):
     del junk
     _, m, r = ops.layernorm_forward(torch.empty(64, 64, 0, device="cuda"))
     assert m.shape == r.shape == (64, 64) and bool(torch.isnan(m).all()) and bool(torch.isnan(r).all())
+
+
+# ---- tensors beside and over one another ------------------------------------------------------------------------
+def adjacent(*shapes):
+    """fp32 tensors one behind another in one buffer."""
+    sizes = [torch.Size(s).numel() for s in shapes]
+    buf = torch.zeros(sum(sizes), device="cuda")
+    return [t.view(s) for t, s in zip(buf.split(sizes), shapes)]
+
+
+def test_layernorm_of_tensors_side_by_side(ops):
+    """Nothing lies between the tensors, and every call is right. Moved by one element, it is refused."""
+    from cantors_gift_b200 import CgB200Error
+    rows, cols = 29, 100
+    x, dy, gamma, beta = normal(rows, cols, seed=1), normal(rows, cols, seed=2), normal(cols, seed=3), normal(cols, seed=4)
+    want = check_ln_forward(ops, x, gamma, beta)
+    check_ln_backward(ops, dy, x, want[1], want[2], gamma)
+    out, x2, mean, g2, rstd, b2 = adjacent((rows, cols), (rows, cols), (rows,), (cols,), (rows,), (cols,))
+    x2.copy_(x), g2.copy_(gamma), b2.copy_(beta)
+    for a, b in zip(ops.layernorm_forward(x2, g2, b2, out=out, mean=mean, rstd=rstd), want):
+        assert torch.equal(a, b)   # a row's sums do not depend on where the parameters lie
+    dx, dy2, dg, x2, db, m2, g2, r2 = adjacent((rows, cols), (rows, cols), (cols,), (rows, cols), (cols,), (rows,), (cols,), (rows,))
+    x2.copy_(x), dy2.copy_(dy), g2.copy_(gamma), m2.copy_(want[1]), r2.copy_(want[2])
+    ops.layernorm_backward(dy2, x2, m2, r2, g2, dx=dx, dgamma=dg, dbeta=db)
+    for t, v in ((x2, x), (dy2, dy), (g2, gamma), (m2, want[1]), (r2, want[2])):
+        assert torch.equal(t, v)
+    # where gamma lies decides how many CTAs take the rows and so the order of the sums over them: held to the definition
+    wx, wg, wb = ln_backward_reference(dy, x, want[1], want[2], gamma)
+    h, g = (x.double() - want[1].double()[:, None]).abs() * want[2].double()[:, None], dy.double().abs() * gamma.double().abs()
+    size = x.double().abs() * want[2].double()[:, None] + h
+    assert_within(dg, wg, (dy.double().abs() * size).sum(0), "dgamma")
+    assert_within(db, wb, dy.double().abs().sum(0), "dbeta")
+    assert_within(dx, wx, want[2].double()[:, None] * (g + g.mean(1, keepdim=True) + size * (g * size).mean(1, keepdim=True)), "dx")
+    buf = torch.zeros(2 * rows * cols, device="cuda")
+    at = lambda i: buf[i:i + rows * cols].view(rows, cols)
+    for bad in (lambda: ops.layernorm_forward(at(0), out=at(1)), lambda: ops.layernorm_forward(at(5), out=at(0)),
+                lambda: ops.layernorm_backward(at(0), x, mean, rstd, dx=at(cols)), lambda: ops.layernorm_backward(dy, at(4), mean, rstd, dx=at(0)),
+                lambda: ops.layernorm_backward(dy, x, want[1], want[2], gamma, dgamma=g2, dbeta=g2)):
+        with pytest.raises(CgB200Error):
+            bad()

@@ -1,0 +1,43 @@
+"""Calls of the training operators that their documentation rules out, decided on the host before a device is touched."""
+import ctypes as C
+
+import pytest
+
+AT = 1 << 20   # an address that is never read
+
+
+def test_layernorm_forward_overlaps(cgb):
+    """4 x 8 bf16 rows (64 bytes), fp32 parameters (32 bytes), statistics of 16 bytes."""
+    capi, L = cgb.capi, cgb.lib()
+    place = dict(x=AT, gamma=AT + 256, beta=AT + 512, y=AT + 768, mean=AT + 1024, rstd=AT + 1280)
+
+    def call(**moved):
+        a = {**place, **moved}
+        return L.cg_b200_layernorm_forward(capi.BF16, capi.F32, *(C.c_void_p(a[k]) for k in ("x", "gamma", "beta")), 1e-5,
+                                           *(C.c_void_p(a[k]) for k in ("y", "mean", "rstd")), 4, 8, None)
+
+    bad = [dict(y=AT + 2), dict(y=AT - 2), dict(y=AT + 62), dict(y=AT - 62), dict(y=AT + 256), dict(y=AT + 286), dict(y=AT + 512 - 62),
+           dict(y=AT + 1024), dict(y=AT + 1280 + 14), dict(mean=AT), dict(mean=AT + 60), dict(mean=AT + 256), dict(mean=AT + 512 + 28),
+           dict(mean=AT + 1280), dict(rstd=AT), dict(rstd=AT + 256 - 12), dict(rstd=AT + 512), dict(rstd=AT + 1024 + 12), dict(rstd=AT + 768)]
+    for moved in bad:
+        assert call(**moved) == capi.ERR_INVALID_ARG, moved
+
+
+def test_layernorm_backward_overlaps(cgb):
+    capi, L = cgb.capi, cgb.lib()
+    need = C.c_size_t(0)
+    assert L.cg_b200_layernorm_backward_workspace_bytes(4, 8, C.byref(need)) == capi.OK
+    names = ("dy", "x", "gamma", "mean", "rstd", "dx", "dgamma", "dbeta")
+    place = {k: AT + 256 * i for i, k in enumerate(names)}
+    place["ws"] = AT + 4096
+
+    def call(**moved):
+        a = {**place, **moved}
+        return L.cg_b200_layernorm_backward(capi.BF16, capi.F32, *(C.c_void_p(a[k]) for k in names), 4, 8, C.c_void_p(a["ws"]), need, None)
+
+    bad = [dict(dx=place[k] + d) for k, d in (("dy", 2), ("dy", -62), ("x", -2), ("x", 62), ("gamma", 0), ("gamma", 30), ("mean", 0), ("rstd", 14),
+                                              ("dgamma", -62), ("dbeta", 0), ("ws", 0))]
+    bad += [dict(dgamma=place["dbeta"] + 28), dict(dbeta=place["dgamma"]), dict(dbeta=place["dx"] + 60)]
+    bad += [dict(ws=place[k] // 16 * 16) for k in names] + [dict(ws=AT + 16 - need.value // 16 * 16)]
+    for moved in bad:
+        assert call(**moved) == capi.ERR_INVALID_ARG, moved
