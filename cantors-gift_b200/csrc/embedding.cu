@@ -921,6 +921,8 @@ extern "C" int cg_b200_embedding(int dtype, int table_dtype, const void* table, 
     if ((!table && vocab > 0) || !ids || !out) return CG_B200_ERR_NULL_POINTER;
     if (!aligned_to(table, dtype_bytes(table_dtype)) || !aligned_to(ids, id_bytes) || !aligned_to(out, dtype_bytes(dtype)))
         return CG_B200_ERR_MISALIGNED;
+    if (overlaps_any(Bytes(out, n * cols, dtype_bytes(dtype)), Bytes(table, vocab * cols, dtype_bytes(table_dtype)), Bytes(ids, n, id_bytes)))
+        return CG_B200_ERR_INVALID_ARG;
     int st = require_sm100();
     if (st) return st;
     const EmbParams p{table, ids, out, n, vocab, cols, scale};
@@ -961,6 +963,10 @@ extern "C" int cg_b200_embedding_backward(int dtype, int grad_dtype, const void*
         return CG_B200_ERR_MISALIGNED;
     const EmbWorkspace w = emb_workspace(n, vocab, cols);
     if (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes)) return CG_B200_ERR_WORKSPACE;
+    // rows of the table are cleared beside the sort, before dout is read
+    const Bytes dy(dout, n * cols, dtype_bytes(dtype)), dt(dtable, vocab * cols, dtype_bytes(grad_dtype)), id(ids, n, id_bytes),
+        scratch(workspace, (int64_t)w.bytes, 1);
+    if (overlaps_any(dt, dy, id) || overlaps_any(scratch, dy, dt, id)) return CG_B200_ERR_INVALID_ARG;
     int st = require_sm100();
     if (st) return st;
     cudaStream_t s = (cudaStream_t)stream;

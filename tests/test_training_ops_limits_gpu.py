@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_training_ops_gpu import CHAIN, DTYPES, assert_within, check_ln_backward, check_ln_forward, guarded, ln_backward_reference, normal
+from test_training_ops_gpu import CHAIN, DTYPES, assert_within, check_ln_backward, check_ln_forward, guarded, ln_backward_reference, normal, embedding_grad_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -186,5 +186,25 @@ def test_layernorm_of_tensors_side_by_side(ops):
     for bad in (lambda: ops.layernorm_forward(at(0), out=at(1)), lambda: ops.layernorm_forward(at(5), out=at(0)),
                 lambda: ops.layernorm_backward(at(0), x, mean, rstd, dx=at(cols)), lambda: ops.layernorm_backward(dy, at(4), mean, rstd, dx=at(0)),
                 lambda: ops.layernorm_backward(dy, x, want[1], want[2], gamma, dgamma=g2, dbeta=g2)):
+        with pytest.raises(CgB200Error):
+            bad()
+
+
+def test_embedding_of_tensors_side_by_side(ops):
+    from cantors_gift_b200 import CgB200Error
+    n, vocab, cols = 40, 30, 33
+    table, dy = normal(vocab, cols, seed=1), normal(n, cols, seed=2)
+    ids = torch.arange(n, device="cuda") % vocab
+    out, t2, grad, dy2 = adjacent((n, cols), (vocab, cols), (vocab, cols), (n, cols))
+    t2.copy_(table), dy2.copy_(dy)
+    assert torch.equal(ops.embedding(t2, ids, out=out), table[ids])
+    got = ops.embedding_backward(dy2, ids, vocab, out=grad)
+    assert torch.equal(t2, table) and torch.equal(dy2, dy) and torch.equal(out, table[ids])
+    want, size, count = embedding_grad_reference(dy, ids, vocab, 1.0)
+    assert_within(got, want, size, "gradient", chain=64 * 2.0 ** -24)
+    square = torch.zeros(n * cols + 1, device="cuda")
+    at = lambda i: square[i:i + n * cols].view(n, cols)
+    for bad in (lambda: ops.embedding(at(0), ids, out=at(0)), lambda: ops.embedding(at(0), ids, out=at(1)),
+                lambda: ops.embedding_backward(at(0), ids, n, out=at(0)), lambda: ops.embedding_backward(at(1), ids, n, out=at(0), accumulate=True)):
         with pytest.raises(CgB200Error):
             bad()

@@ -41,3 +41,28 @@ def test_layernorm_backward_overlaps(cgb):
     bad += [dict(ws=place[k] // 16 * 16) for k in names] + [dict(ws=AT + 16 - need.value // 16 * 16)]
     for moved in bad:
         assert call(**moved) == capi.ERR_INVALID_ARG, moved
+
+
+def test_embedding_overlaps(cgb):
+    """A table of 10 rows of 8 fp32 (320 bytes), 4 ids of 8 bytes, 4 rows of 8 bf16 (64 bytes)."""
+    capi, L = cgb.capi, cgb.lib()
+    table, ids, rows = AT, AT + 512, AT + 768
+
+    def lookup(out):
+        return L.cg_b200_embedding(capi.BF16, capi.F32, C.c_void_p(table), 10, 8, C.c_void_p(ids), 8, 4, 1.0, C.c_void_p(out), None)
+
+    for out in (table, table - 62, table + 318, ids, ids - 62, ids + 30):
+        assert lookup(out) == capi.ERR_INVALID_ARG, out - AT
+
+    need = C.c_size_t(0)
+    assert L.cg_b200_embedding_backward_workspace_bytes(4, 10, 8, C.byref(need)) == capi.OK
+    place = dict(dy=rows, ids=ids, dtable=table, ws=AT + 4096)
+
+    def gradient(accumulate=0, **moved):
+        a = {k: C.c_void_p(v) for k, v in {**place, **moved}.items()}
+        return L.cg_b200_embedding_backward(capi.BF16, capi.F32, a["dy"], a["ids"], 8, 4, 1.0, -1, accumulate, a["dtable"], 10, 8, a["ws"], need, None)
+
+    for moved in (dict(dy=table), dict(dy=table + 318), dict(dy=table - 62), dict(ids=table + 312), dict(dtable=rows + 60), dict(dtable=ids - 316),
+                  dict(ws=AT), dict(ws=AT + 512), dict(ws=AT + 768), dict(dtable=AT + 4096 + need.value - 4), dict(dy=AT + 4096 - 62)):
+        for accumulate in (0, 1):
+            assert gradient(accumulate, **moved) == capi.ERR_INVALID_ARG, moved
