@@ -326,6 +326,13 @@ static int clip_entry(const cg_b200_grad* grads, int64_t count, float max_norm, 
     if (!norm) return CG_B200_ERR_NULL_POINTER;
     if (!aligned_to(norm, 4) || !aligned_to(workspace, 16)) return CG_B200_ERR_MISALIGNED;
     if (!workspace || workspace_bytes < clip_workspace(count)) return CG_B200_ERR_WORKSPACE;
+    // sums are written there while the list is read, and read while it and the norm are written
+    const Bytes ws(workspace, (int64_t)clip_workspace(count), 1);
+    bool bad = overlap(ws, Bytes(norm, 1, sizeof(float)));
+    for (int64_t i = 0; i < count; ++i)
+        bad |= overlap(ws, Bytes(grads[i].in, grads[i].n, dtype_bytes(grads[i].dtype))) ||
+               (scale && overlap(ws, Bytes(grads[i].out, grads[i].n, dtype_bytes(grads[i].out_dtype))));
+    if (bad) return CG_B200_ERR_INVALID_ARG;
     st = require_sm100();
     if (st) return st;
     return clip_run(grads, count, max_norm, norm, static_cast<double*>(workspace), scale, (cudaStream_t)stream);

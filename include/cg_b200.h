@@ -264,7 +264,7 @@ int cg_b200_reduce(int dtype, int op, const void* in, void* out, int64_t outer, 
  * any input. No tensor may be written twice, and *norm (fp32 on the device) is part of none. Squares are summed in fp64
  * beyond 16-byte packets, in a fixed order; a list whose norm is infinite or not a number is scaled by the factor that the
  * formula gives (0 or NaN). cg_b200_grad_norm ignores out, out_dtype. count <= 2^20; count == 0 gives norm 0. The workspace
- * must be 16-byte aligned; two calls that can run at the same time need one each. */
+ * must be 16-byte aligned and apart from the tensors and *norm; two calls that can run at the same time need one each. */
 typedef struct cg_b200_grad {
     const void* in;
     void*       out;

@@ -66,3 +66,27 @@ def test_embedding_overlaps(cgb):
                   dict(ws=AT), dict(ws=AT + 512), dict(ws=AT + 768), dict(dtable=AT + 4096 + need.value - 4), dict(dy=AT + 4096 - 62)):
         for accumulate in (0, 1):
             assert gradient(accumulate, **moved) == capi.ERR_INVALID_ARG, moved
+
+
+def test_clip_workspace_apart_from_the_list(cgb):
+    capi, L = cgb.capi, cgb.lib()
+    need = C.c_size_t(0)
+    assert L.cg_b200_grad_norm_workspace_bytes(2, C.byref(need)) == capi.OK
+    t = (capi.Grad * 2)()
+    for i, e in enumerate(t):
+        e.in_, e.out, e.n, e.dtype, e.out_dtype = AT + i * 4096, AT + 16384 + i * 4096, 100, capi.BF16, capi.F32
+    far = AT + (1 << 20)
+
+    def clip(ws, norm=far):
+        return L.cg_b200_clip_grad_norm(t, 2, 1.0, C.c_void_p(norm), C.c_void_p(ws), need, None)
+
+    def norm_only(ws, norm=far):
+        return L.cg_b200_grad_norm(t, 2, C.c_void_p(norm), C.c_void_p(ws), need, None)
+
+    before = need.value // 16 * 16
+    for at in (AT, AT + 192, AT + 4096 + 192, AT - before + 16):
+        assert clip(at) == norm_only(at) == capi.ERR_INVALID_ARG, at - AT
+    for at in (AT + 16384 + 384, AT + 20480 + 384, AT + 20480):
+        assert clip(at) == capi.ERR_INVALID_ARG, at - AT
+    for at in (far, far + need.value - 4):
+        assert clip(far, norm=at) == norm_only(far, norm=at) == capi.ERR_INVALID_ARG
