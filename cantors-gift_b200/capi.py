@@ -11,6 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 OK = 0
 ERR_INVALID_ARG, ERR_NULL_POINTER, ERR_MISALIGNED, ERR_UNSUPPORTED, ERR_CUDA = 1, 2, 3, 4, 5
 ERR_NO_DEVICE, ERR_WORKSPACE, ERR_DEVICE_TIMEOUT, ERR_COMM, ERR_FUSED_IR, ERR_NOT_SM100 = 6, 7, 8, 9, 10, 11
+ERR_NO_MEMORY = 12
 
 F16, BF16, F32 = 0, 1, 2
 DTYPE_BYTES = {F16: 2, BF16: 2, F32: 4}

@@ -226,7 +226,7 @@ struct ClipRange {
 static int clip_check_overlap(const cg_b200_grad* g, int64_t count, const float* norm) {
     ClipRange few[2 * kClipShort + 1];
     ClipRange* r = few;
-    if (count > kClipShort && !(r = static_cast<ClipRange*>(malloc(((size_t)count * 2 + 1) * sizeof(ClipRange))))) return CG_B200_ERR_INVALID_ARG;
+    if (count > kClipShort && !(r = static_cast<ClipRange*>(malloc(((size_t)count * 2 + 1) * sizeof(ClipRange))))) return CG_B200_ERR_NO_MEMORY;
     int64_t n = 0;
     if (norm) r[n++] = {reinterpret_cast<uintptr_t>(norm), reinterpret_cast<uintptr_t>(norm) + sizeof(float), true};
     for (int64_t i = 0; i < count; ++i) {

@@ -91,6 +91,7 @@ const char* cg_b200_status_string(int status) {
         case CG_B200_ERR_COMM: return "NCCL failure";
         case CG_B200_ERR_FUSED_IR: return "IR carries lossy fusion markers (fused_chain / fused_with)";
         case CG_B200_ERR_NOT_SM100: return "device is not compute capability 10.x";
+        case CG_B200_ERR_NO_MEMORY: return "out of host memory";
         default: return "unknown status";
     }
 }

@@ -42,7 +42,8 @@ enum cg_b200_status {
     CG_B200_ERR_DEVICE_TIMEOUT = 8, /* a bounded device-side wait ran out                */
     CG_B200_ERR_COMM = 9,           /* NCCL failure                                      */
     CG_B200_ERR_FUSED_IR = 10,      /* IR carries the reference's lossy fusion markers   */
-    CG_B200_ERR_NOT_SM100 = 11      /* device is not compute capability 10.x             */
+    CG_B200_ERR_NOT_SM100 = 11,     /* device is not compute capability 10.x             */
+    CG_B200_ERR_NO_MEMORY = 12      /* host memory that the call needs cannot be had     */
 };
 
 /* Element types. Numbering equals the reference's cg::DType (include/cg/core/dtype.hpp:14-40). */
@@ -263,8 +264,8 @@ int cg_b200_reduce(int dtype, int op, const void* in, void* out, int64_t outer, 
  * size; out_dtype is `dtype` or CG_B200_F32, out may be `in` itself when the types agree and otherwise must not overlap
  * any input. No tensor may be written twice, and *norm (fp32 on the device) is part of none. Squares are summed in fp64
  * beyond 16-byte packets, in a fixed order; a list whose norm is infinite or not a number is scaled by the factor that the
- * formula gives (0 or NaN). cg_b200_grad_norm ignores out, out_dtype. count <= 2^20; count == 0 gives norm 0. The workspace
- * must be 16-byte aligned and apart from the tensors and *norm; two calls that can run at the same time need one each. */
+ * formula gives (0 or NaN). cg_b200_grad_norm ignores out, out_dtype. count <= 2^20; count == 0 gives norm 0. Clipping
+ * more than 64 tensors takes 48 bytes of host memory for each during the call (CG_B200_ERR_NO_MEMORY). The workspace must be 16-byte aligned and apart from the tensors and *norm; two calls that can run at the same time need one each. */
 typedef struct cg_b200_grad {
     const void* in;
     void*       out;

@@ -1,7 +1,9 @@
 """Calls of the training operators that their documentation rules out, decided on the host before a device is touched."""
 import ctypes as C
+import subprocess
+import sys
 
-import pytest
+from conftest import ROOT
 
 AT = 1 << 20   # an address that is never read
 
@@ -90,3 +92,26 @@ def test_clip_workspace_apart_from_the_list(cgb):
         assert clip(at) == capi.ERR_INVALID_ARG, at - AT
     for at in (far, far + need.value - 4):
         assert clip(far, norm=at) == norm_only(far, norm=at) == capi.ERR_INVALID_ARG
+
+
+def test_clip_without_host_memory(cgb):
+    """A list of 2^20 tensors takes 48 MB on the host for its address ranges; a process that may not have them is told so."""
+    code = """
+import ctypes as C, resource
+from cantors_gift_b200 import capi
+L = capi.lib()
+count = 1 << 20
+t = (capi.Grad * count)()
+for i, e in enumerate(t):
+    e.in_ = e.out = (1 << 30) + i * 64
+    e.n, e.dtype, e.out_dtype = 16, capi.F32, capi.F32
+clip = lambda: L.cg_b200_clip_grad_norm(t, count, 1.0, C.c_void_p(1 << 20), None, 0, None)
+assert clip() == capi.ERR_WORKSPACE, "with memory"
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (16 << 20),) * 2)
+assert clip() == capi.ERR_NO_MEMORY, "without"
+assert L.cg_b200_status_string(capi.ERR_NO_MEMORY) == b"out of host memory"
+print("refused")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "refused" in r.stdout, r.stdout + r.stderr
