@@ -882,15 +882,21 @@ static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long 
     return CG_B200_OK;
 }
 
+// Column tiles of a row of packets of `packet` elements, and whether a grid holds all chunks' tiles and the blocks that clear
+constexpr long long kZeroBlocks = 1 << 20;   // of those at most
+static long long emb_tiles(long long cols, int packet) { return (cols + 32 * packet - 1) / (32 * packet); }
+static bool emb_grid_ok(long long chunks, long long cols, int dtype) {
+    return chunks * emb_tiles(cols, 16 / (int)dtype_bytes(dtype)) <= 0x7fffffffll - kZeroBlocks;
+}
+
 template <typename T, typename G>
 static int emb_backward(EmbGradParams p, cudaStream_t s) {
     constexpr int L = Vec16<T>::N;
     const bool vec = p.cols % L == 0 && aligned_to(p.dout, 16) && aligned_to(p.dtable, 16);
-    p.tiles = (int)((p.cols + 32 * L - 1) / (32 * L));
-    const long long zero_cap = (long long)sm_count() * 256 / kEmbWarps, want = (p.zero_rows + kEmbWarps * kZeroRows - 1) / (kEmbWarps * kZeroRows);
+    p.tiles = (int)emb_tiles(p.cols, L);
+    const long long most = (long long)sm_count() * 256 / kEmbWarps, zero_cap = most < kZeroBlocks ? most : kZeroBlocks, want = (p.zero_rows + kEmbWarps * kZeroRows - 1) / (kEmbWarps * kZeroRows);
     p.zero_blocks = (int)(want < zero_cap ? want : zero_cap);
-    const long long blocks = (p.chunks * p.tiles + kEmbWarps - 1) / kEmbWarps + p.zero_blocks;
-    if (blocks > 0x7fffffffll) return CG_B200_ERR_UNSUPPORTED;
+    const long long blocks = (p.chunks * p.tiles + kEmbWarps - 1) / kEmbWarps + p.zero_blocks;   // fit a grid, see emb_grid_ok
     auto k = vec ? emb_grad_kernel<T, G, true> : emb_grad_kernel<T, G, false>;
     const int smem = kEmbWarps * kEmbGroups * kEmbRows * (vec ? 32 : 33) * 16;
     if (blocks > 0) {
@@ -962,6 +968,7 @@ extern "C" int cg_b200_embedding_backward(int dtype, int grad_dtype, const void*
         !aligned_to(workspace, 256))
         return CG_B200_ERR_MISALIGNED;
     const EmbWorkspace w = emb_workspace(n, vocab, cols);
+    if (!emb_grid_ok(w.chunks, cols, dtype)) return CG_B200_ERR_UNSUPPORTED;
     if (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes)) return CG_B200_ERR_WORKSPACE;
     // rows of the table are cleared beside the sort, before dout is read
     const Bytes dy(dout, n * cols, dtype_bytes(dtype)), dt(dtable, vocab * cols, dtype_bytes(grad_dtype)), id(ids, n, id_bytes),

@@ -235,7 +235,8 @@ int cg_b200_layernorm_backward(int dtype, int param_dtype, const void* dout, con
  * out / dout are `dtype`; table is `table_dtype`, dtable `grad_dtype`, each `dtype` or CG_B200_F32. All contiguous, any
  * alignment down to the element size; 16-byte packets are used when cols and the bases allow them. The sums are fp32 in
  * an order that the ids alone decide (the same inputs give the same bits on every call), rounded once.
- * n <= 2^31 - 1, vocab < 2^31 - 1, cols <= 2^30. out, dtable and the workspace overlap nothing else of the call
+ * n <= 2^31 - 1, vocab < 2^31 - 1, cols <= 2^30; a dout whose pieces of 32 rows by 512 bytes are more than 2^31 - 2^20 - 1
+ * in number is refused (CG_B200_ERR_UNSUPPORTED; more than any memory holds). out, dtable and the workspace overlap nothing else of the call
  * (CG_B200_ERR_INVALID_ARG). The workspace must be 256-byte aligned; its contents are undefined before and after, and two
  * calls that can run at the same time need one each. */
 int cg_b200_embedding(int dtype, int table_dtype, const void* table, int64_t vocab, int64_t cols, const void* ids,

@@ -70,6 +70,23 @@ def test_embedding_overlaps(cgb):
             assert gradient(accumulate, **moved) == capi.ERR_INVALID_ARG, moved
 
 
+def test_embedding_gradient_of_too_many_pieces(cgb):
+    """More blocks than a grid has are refused before anything is launched: 2^26 chunks of 32 ids, 32 or more tiles of 512 bytes."""
+    capi, L = cgb.capi, cgb.lib()
+
+    def call(dtype, cols, n=(1 << 31) - 1, ws=1 << 62):
+        need = C.c_size_t(0)
+        assert L.cg_b200_embedding_backward_workspace_bytes(n, 10, cols, C.byref(need)) == capi.OK
+        return L.cg_b200_embedding_backward(dtype, capi.F32, C.c_void_p(1 << 60), C.c_void_p(1 << 59), 8, n, 1.0, -1, 0, C.c_void_p(1 << 58), 10, cols,
+                                            C.c_void_p(ws), need, None)
+
+    for dtype, tile in ((capi.F32, 128), (capi.BF16, 256), (capi.F16, 256)):
+        assert call(dtype, 32 * tile) == capi.ERR_UNSUPPORTED
+        assert call(dtype, 1 << 30) == capi.ERR_UNSUPPORTED
+        assert call(dtype, 31 * tile, ws=None) == capi.ERR_WORKSPACE           # fits
+        assert call(dtype, 31 * tile + 1) == capi.ERR_UNSUPPORTED
+
+
 def test_clip_workspace_apart_from_the_list(cgb):
     capi, L = cgb.capi, cgb.lib()
     need = C.c_size_t(0)
