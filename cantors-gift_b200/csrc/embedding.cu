@@ -479,8 +479,10 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __g
 // 120 MB beside it took 37 us, with 78 MB 21, with none 21)
 constexpr long long kZeroBase = 30, kZeroPerRound = 12;
 
+// *placed: whether it was launched. Where no cluster of so many CTAs finds room at all (a partition of a GPU with few SMs to a GPC), it is not,
+// and the launches over all ids sort them.
 template <typename I, int ROUNDS>
-static cudaError_t sort_cluster(const SortParams& p, int passes, int digit_bits, int ctas, cudaStream_t s) {
+static cudaError_t sort_cluster(const SortParams& p, int passes, int digit_bits, int ctas, bool* placed, cudaStream_t s) {
     auto k = sort_cluster_kernel<I, ROUNDS>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared<ROUNDS>));
     if (e == cudaSuccess && ctas > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -498,6 +500,12 @@ static cudaError_t sort_cluster(const SortParams& p, int passes, int digit_bits,
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    int clusters = 0;
+    *placed = ctas == 1 || (cudaOccupancyMaxActiveClusters(&clusters, k, &cfg) == cudaSuccess && clusters > 0);
+    if (!*placed) {
+        cudaGetLastError();   // the answer may be an error; it is nobody else's
+        return cudaSuccess;
+    }
     return cudaLaunchKernelEx(&cfg, k, p, passes, digit_bits);
 }
 
@@ -851,19 +859,22 @@ static int emb_sort(const EmbWorkspace& w, char* ws, const void* ids, long long 
         int ctas = 1, rounds = 1;
         while (ctas < 16 && ctas * kRound < n) ctas *= 2;
         while (rounds * ctas * kRound < n) rounds *= 2;
-        *result = 0;
         // rows to clear meanwhile: what memory takes in the time of the sort
         const long long fit = ((kZeroBase + kZeroPerRound * rounds) << 20) / row_bytes, rows = fit < *zero_rows ? fit : *zero_rows;
-        *zero_rows -= rows;
-        p.zero_from = static_cast<char*>(dtable) + *zero_rows * row_bytes;
+        p.zero_from = static_cast<char*>(dtable) + (*zero_rows - rows) * row_bytes;
         p.zero_bytes = rows * row_bytes;
+        bool placed = false;
         switch (rounds) {
-            case 1: CGB_CUDA((sort_cluster<I, 1>(p, w.passes, w.digit_bits, ctas, s))); break;
-            case 2: CGB_CUDA((sort_cluster<I, 2>(p, w.passes, w.digit_bits, ctas, s))); break;
-            case 4: CGB_CUDA((sort_cluster<I, 4>(p, w.passes, w.digit_bits, ctas, s))); break;
-            default: CGB_CUDA((sort_cluster<I, 8>(p, w.passes, w.digit_bits, ctas, s)));
+            case 1: CGB_CUDA((sort_cluster<I, 1>(p, w.passes, w.digit_bits, ctas, &placed, s))); break;
+            case 2: CGB_CUDA((sort_cluster<I, 2>(p, w.passes, w.digit_bits, ctas, &placed, s))); break;
+            case 4: CGB_CUDA((sort_cluster<I, 4>(p, w.passes, w.digit_bits, ctas, &placed, s))); break;
+            default: CGB_CUDA((sort_cluster<I, 8>(p, w.passes, w.digit_bits, ctas, &placed, s)));
         }
-        return CG_B200_OK;
+        if (placed) {
+            *zero_rows -= rows;
+            *result = 0;
+            return CG_B200_OK;
+        }
     }
     p.count = reinterpret_cast<uint32_t*>(ws + w.count);
     int cur = 0;
