@@ -2,15 +2,15 @@
 //
 // The reference has no such operator on its executed path; the encoder block here takes activations, and this is what makes them.
 //   forward   out[n] = scale * table[id[n]]
-//   backward  dtable[v] = scale * (sum of dout[n] over the n with id[n] == v, in the order of n)
+//   backward  dtable[v] = scale * (sum of dout[n] over the n with id[n] == v)
 // An id outside [0, vocab) selects nothing: its output row is zero and its gradient is dropped, as is the padding id's gradient.
 //
 // Both are HBM-bound. Forward moves the rows that occur (L2 serves repeats) and the output. Backward reads dout once and writes the table
-// once. It sorts the (id, n) pairs by id - a stable radix sort, so equal ids stay in the order of n and the sums do not depend on
-// timing - and walks the sorted list in chunks of 32 pairs. A warp takes a chunk for 512 bytes of columns: it adds the rows of every id
+// once. It sorts the (id, n) pairs by id - a stable radix sort, so equal ids stay in the order of n, and the ids alone decide in what
+// order rows are added, never the timing - and walks the sorted list in chunks of 32 pairs. A warp takes a chunk for 512 bytes of columns: it adds the rows of every id
 // that begins in the chunk, in fp32 registers, following the last one into the next chunk, and writes the id's table row. Only an id
 // whose pairs cover a whole chunk and reach beyond it is added by several warps: their sums go to the workspace and a last kernel joins
-// them in order. The table rows that no id names are cleared beside the sort, as far as that takes no longer than the sort, and beside
+// them, in eight strands of every eighth chunk. The table rows that no id names are cleared beside the sort, as far as that takes no longer than the sort, and beside
 // the sums.
 #include <cooperative_groups.h>
 
@@ -476,7 +476,8 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __g
 }
 
 // MB cleared beside a sort of so many rounds: what the six or so other clusters that find room write in its time (a sort of four rounds with
-// 120 MB beside it took 37 us, with 78 MB 21, with none 21)
+// 120 MB beside it took 37 us, with 78 MB 21, with none 21). Four rounds are the one point measured; the line through it for one, two and
+// eight rounds is an estimate.
 constexpr long long kZeroBase = 30, kZeroPerRound = 12;
 
 // *placed: whether it was launched. Where no cluster of so many CTAs finds room at all (a partition of a GPU with few SMs to a GPC), it is not,

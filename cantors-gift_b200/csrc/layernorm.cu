@@ -6,15 +6,16 @@
 //   backward  dx = rstd * (g - sum(g) / C - h * sum(g * h) / C)         (the two sums over the row)
 //             dgamma = sum over rows of dy * h,  dbeta = sum over rows of dy
 //
-// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once (measured: 65536 x 1024 bf16 forward 49 us, 84 % of the copy
-// rate; 32768 x 4096 bf16 backward 129 - 134 us, 92 - 95 %; 14000 x 8000 fp32 148 and 212 us, 92 and 97 %). One CTA per SM
+// HBM-bound: forward moves 2 * R * C elements, backward 3 * R * C, each once (measured: 65536 x 1024 bf16 forward 48 us, 85 % of the copy
+// rate; 32768 x 4096 bf16 backward 135 us, 91 %; 14000 x 8000 fp32 147 and 215 us, 93 and 95 %). One CTA per SM
 // walks the rows; its threads form groups, a row (forward: two rows at once) to a group: eight threads, a warp, or up to 16 warps with a
 // barrier of their own. A row is 16-byte packets, packet j * TPR + t for thread t, copied asynchronously into shared memory ahead of
 // its use: a thread copies and reads its own packets only, so nothing but its own copies has to be waited for, and loads stay in flight
 // while rows are reduced without costing registers (loads into registers, with a row's lookahead: 59 and 229 us). In the backward pass
 // each thread adds its columns' share of dgamma and dbeta to fp32 registers over all rows of its group; the groups' sums are joined in
 // shared memory, the CTAs' sums go to the workspace and a second kernel adds them up, all in a fixed order, so the result does not
-// depend on timing. Arithmetic is on fp32 pairs: with single instructions the backward
+// depend on timing. (A group's running sum takes rows / (148 * groups) terms, 110 for 32768 x 4096 bf16; the register kernels' error in
+// dgamma and dbeta grows with that, the streaming kernels' does not.) Arithmetic is on fp32 pairs: with single instructions the backward
 // pass is bound by issue before it is bound by HBM.
 //
 // Rows whose width no packet divides start at a different offset from a 16-byte boundary each. The rows of one CTA are gridDim.x apart, a
@@ -795,7 +796,8 @@ static int ln_launch(const LnParams& p, bool ragged, int* parts, cudaStream_t s)
     // rows are reduced. The short rows of SUB take three (524288 x 64 bf16 forward 27.4 us, with two 30.6). 16-bit rows, which compute twice
     // as much per byte, take two (65536 x 1024 bf16 forward 49.5 us, with three 51.7; 24576 x 4096 69 us, with one 74). fp32 rows take
     // one where enough threads have rows (24576 x 4096 forward 133 us and backward 192, with two 137 and 203; 16000 x 2500 backward 82 and 93),
-    // two where one group leaves many threads out (6000 x 5000, 320 threads: forward 43 us and backward 63, with one 48 and 72).
+    // two where one group leaves many threads out (6000 x 5000, 320 threads: forward 43 us and backward 63, with one 48 and 72). The borders
+    // at 352 and 448 threads lie between the shapes named here; nothing nearer to them was measured.
     const bool one = sizeof(T) == 4 && (sh.groups > 1 || threads >= (BWD ? 448 : 352));
     sh.stages = SUB ? 3 : one ? 1 : 2;
     while (row * sh.stages > kLnSmem) --sh.stages;

@@ -209,7 +209,8 @@ int cg_b200_softmax_layernorm(int dtype, const void* in, const void* gamma,
  * in, dout, out, din are [rows, cols] row-major contiguous of `dtype`; gamma, beta, dgamma, dbeta are [cols] of
  * `param_dtype`, which is `dtype` or CG_B200_F32; mean, rstd are [rows] fp32. Any alignment down to the element size is
  * taken; 16-byte packets are used when the [rows, cols] tensors start at the same offset from a 16-byte boundary. Math
- * and sums are fp32, one rounding per result; the same inputs give the same bits on every call.
+ * and sums are fp32 (beyond runs of 64 terms fp64 where that packet rule or rows of more than 16384 columns leave no
+ * packets), one rounding per result; the same inputs at the same alignment give the same bits on every call.
  * cols == 0: both do nothing, so mean and rstd stay as they are.
  * Forward: gamma, beta, mean, rstd may be NULL. out may be `in` itself; apart from that out, mean and rstd overlap neither
  * an input nor one another (CG_B200_ERR_INVALID_ARG).
@@ -258,7 +259,8 @@ int cg_b200_reduce(int dtype, int op, const void* in, void* out, int64_t outer, 
                    int64_t inner, void* stream);
 
 /* ---- gradient norm and clipping over a list of tensors ------------------------------------
- * The reference's reductions take one tensor; these take a model's whole gradient list in a fixed number of launches.
+ * The reference's reductions take one tensor; these take a model's whole gradient list, 448 tensors to a launch of each
+ * of the two passes.
  *   norm = sqrt(sum over all tensors and elements of in^2)
  *   clip: out = in * min(1, max_norm / (norm + 1e-6)), each rounded once to out_dtype
  * `host_grads` is read before the call returns. A tensor is `n` contiguous elements of any alignment down to its element
