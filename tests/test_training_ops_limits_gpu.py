@@ -78,6 +78,43 @@ def test_layernorm_graph_of_two_sizes_replays(ops):
             assert torch.equal(a, b)
 
 
+def test_embedding_and_clipping_from_host_threads(ops):
+    """The same for the embedding, its gradient (sorts by one CTA, by clusters of two and sixteen, and by launches over all ids) and clipping."""
+    sizes = [(900, 300, 64), (2000, 5000, 40), (70000, 700, 24), (140000, 3000, 8)]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    sets = [(normal(v, c, seed=n), torch.randint(-1, v, (n,), device="cuda", generator=g), normal(n, c, seed=n + 1)) for n, v, c in sizes]
+
+    def once(table, ids, dy, stream=None):
+        out = ops.embedding(table, ids, scale=2.0, stream=stream)
+        grad = ops.embedding_backward(dy, ids, table.shape[0], scale=2.0, stream=stream)
+        return out, grad, ops.clip_grad_norm([grad, out], 1.0, stream=stream)
+
+    wants = [once(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    start, faults = threading.Barrier(len(sets)), []
+
+    def work(k):
+        try:
+            start.wait()
+            for i in range(100):
+                got = once(*sets[k], stream=streams[k])
+                if i % 10 == 9:
+                    streams[k].synchronize()
+                    for a, b in zip(got, wants[k]):
+                        assert torch.equal(a, b), f"call {i}"
+        except Exception as e:
+            faults.append(f"thread {k}: {e!r}")
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(sets))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not faults, faults
+
+
 # ---- long sums ----------------------------------------------------------------------------------------------
 def steady_rows(rows, cols, dtype, shift):
     """x and dy with the same values in every row: the sums over rows are rows times one term, and the rounding errors of a running sum,
